@@ -48,9 +48,36 @@ def prefix_groups(groups):
     return arr
 
 
+class Rope(C.Structure):
+    """drk_rope: the description of a (stretched) rotary embedding"""
+    _fields_ = [("rotary_dim", C.c_int32), ("interleaved", C.c_int32)] + [(n, C.c_float) for n in (
+        "theta", "factor", "original_positions", "low_turns", "high_turns", "magnitude")]
+
+
+def rope(rotary_dim, interleaved=False, theta=1.0e7, factor=1.0, original_positions=0.0, low_turns=1.0, high_turns=32.0,
+         magnitude=1.0):
+    return Rope(rotary_dim, int(interleaved), theta, factor, original_positions, low_turns, high_turns, magnitude)
+
+
+class RopeRows(C.Structure):
+    """drk_rope_rows: one tensor of head rows"""
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("heads", C.c_int32), ("reserved", C.c_int32)] + [(n, C.c_size_t) for n in (
+        "x_token_stride", "x_head_stride", "out_token_stride", "out_head_stride")]
+
+
+def rope_rows(tensors):
+    """ctypes array of drk_rope_rows from (x, out, heads, x token stride, x head stride, out token stride, out head
+    stride) tuples: addresses, and strides in elements"""
+    arr = (RopeRows * len(tensors))()
+    for i, (x, out, heads, *strides) in enumerate(tensors):
+        arr[i] = RopeRows(x, out, heads, 0, *strides)
+    return arr
+
+
 _vp, _i32, _sz, _f32 = C.c_void_p, C.c_int32, C.c_size_t, C.c_float
 _LP = C.POINTER(Layout)
 _GP = C.POINTER(PrefixGroup)
+_RP, _RRP = C.POINTER(Rope), C.POINTER(RopeRows)
 
 # name -> (restype, argtypes); mirrors include/drk_kv.h and include/drk_debug.h one to one
 SIGNATURES = {
@@ -171,6 +198,17 @@ SIGNATURES = {
                                                     _vp]),
     "drk_importance_update": (_i32, [_vp, _vp, _i32, _f32, _vp]),
     "drk_importance_fold_clear": (_i32, [_vp, _vp, _i32, _f32, _vp]),
+    "drk_rope_freqs_fill": (_i32, [_RP, _vp, _vp]),
+    "drk_rope_table_fill_scaled": (_i32, [_RP, _vp, _i32, _vp]),
+    "drk_rope_apply": (_i32, [_RP, _vp, _RRP, _i32, _i32, _i32, _vp, _i32, _i32, _i32, _vp]),
+    "drk_kv_bounds_bytes": (_sz, [_LP]),
+    "drk_kv_bounds_update": (_i32, [_LP, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "drk_kv_bounds_extract": (_i32, [_LP, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
+    "drk_block_select_workspace_bytes": (_sz, [_LP, _i32, _i32]),
+    "drk_block_select": (_i32, [_LP, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
+    "drk_paged_sparse_workspace_bytes": (_sz, [_LP, _i32, _i32]),
+    "drk_paged_sparse_attention": (_i32, [_LP, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _vp, _i32, _f32, _i32, _vp, _sz, _vp,
+                                          _sz, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,280 @@
+// drk_bounds.hip -- bounds of every block's keys: for each (layer, physical block, kv head) the
+// lowest and highest key per dimension, as int8 codes of one power of two.
+//
+// The code of a bound is floor(low / 2^e) or ceil(high / 2^e) with e from the block's largest
+// magnitude: scaling by a power of two is exact, so the codes follow from the keys alone, without
+// a rounding that could depend on an order.  All of it is HBM-bound: a key row is read once, 2 D + 1
+// bytes come back per block and head.
+#include "drk_common.hpp"
+#include "drk_codec.hpp"
+#include "drk_bounds.hpp"
+
+namespace drk {
+
+constexpr int kBThreads = 256;
+
+struct BoundsArgs {
+    const uint8_t *pool;
+    uint8_t *bounds;
+    const int32_t *tables, *d_pos;
+    size_t exps;                   // offset of the exponents in the buffer
+    int table_stride, pos_start, n, first_block, n_blocks, layer0;
+    unsigned units;                // (layer, block, kv head) triples
+    Div bs_div;
+};
+
+// 16 bytes of a key row as floats
+template <int DT> struct BoundsElems { static constexpr int V = 8; };
+template <> struct BoundsElems<DRK_INT8> { static constexpr int V = 16; };
+template <> struct BoundsElems<DRK_FP8_E4M3> { static constexpr int V = 16; };
+template <int DT>
+__device__ __forceinline__ void bounds_unpack(const uint4 &v, float scale, float *x)
+{
+    if constexpr (DT == DRK_F16 || DT == DRK_BF16) {
+        unpack8(v, DT, x);
+    } else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (DT == DRK_INT8) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) x[4 * i + j] = (float)(int8_t)(w[i] >> (8 * j)) * scale;
+            } else {
+                uint32_t lo, hi;
+                fp8x4_to_f16x4(w[i], lo, hi);
+                x[4 * i] = f16_bits_to_f((uint16_t)(lo & 0xffffu));
+                x[4 * i + 1] = f16_bits_to_f((uint16_t)(lo >> 16));
+                x[4 * i + 2] = f16_bits_to_f((uint16_t)(hi & 0xffffu));
+                x[4 * i + 3] = f16_bits_to_f((uint16_t)(hi >> 16));
+            }
+        }
+    }
+}
+
+// One unit per WPU waves: a row is LPR = row_bytes / 16 consecutive lanes, 64 / LPR rows per wave and load.
+template <int DT, int WPU>
+__global__ __launch_bounds__(kBThreads) void bounds_update_kernel(Lay a, BoundsArgs A, unsigned lpr)
+{
+    constexpr int V = BoundsElems<DT>::V;
+    __shared__ float red[WPU > 1 ? 4 : 1][2][V][64];
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const unsigned unit = WPU > 1 ? blockIdx.x : blockIdx.x * 4 + w;
+    bool ok = unit < A.units;
+    const unsigned h = unit % (unsigned)a.KVH, rest = unit / (unsigned)a.KVH;
+    const unsigned nb = (unsigned)A.n_blocks, bi = rest % nb;
+    const int layer = A.layer0 + (int)(rest / nb);
+    int cnt = 0, blk = -1;
+    if (ok) {
+        int pos, lb;
+        const int32_t *tab = A.tables;
+        if (A.d_pos) {
+            pos = A.d_pos[bi];
+            lb = pos < 0 ? -1 : (int)dv((unsigned)pos, A.bs_div);
+            tab += (size_t)bi * A.table_stride;
+            if (lb >= A.table_stride) lb = -1;
+        } else {
+            lb = A.first_block + (int)bi;
+            pos = A.pos_start + A.n - 1;
+        }
+        if (lb >= 0) {
+            blk = tab[lb];
+            cnt = min(a.bs, pos - lb * a.bs + 1);
+        }
+        ok = blk >= 0 && blk < a.NB;
+    }
+    if (!ok) cnt = 0;
+    const unsigned sub = lane % lpr, r0 = lane / lpr, rpw = 64 / lpr;
+    float lo[V], hi[V];
+#pragma unroll
+    for (int i = 0; i < V; i++) { lo[i] = INFINITY; hi[i] = -INFINITY; }
+    if (ok) {
+        const uint8_t *base = A.pool + row_off(a, layer, blk, 0, (int)h, 0);
+        const uint8_t *sc = A.pool + (DT == DRK_INT8 ? scale_off(a, layer, blk, 0, (int)h, 0) : 0);
+        const int step = (int)rpw * WPU;
+        for (int r = (int)r0 + (WPU > 1 ? w * (int)rpw : 0); r < cnt; r += 4 * step) {
+            uint4 v[4];
+            float s[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                const int rr = min(r + u * step, cnt - 1);         // a row read twice changes no bound
+                v[u] = ld_stream128(base + (size_t)rr * a.row_bytes + sub * 16);
+                s[u] = DT == DRK_INT8 ? f16_bits_to_f(*(const uint16_t *)(sc + (size_t)rr * 2)) : 1.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < 4; u++) {
+                float x[V];
+                bounds_unpack<DT>(v[u], s[u], x);
+#pragma unroll
+                for (int i = 0; i < V; i++) { lo[i] = fminf(lo[i], x[i]); hi[i] = fmaxf(hi[i], x[i]); }
+            }
+        }
+    }
+    for (unsigned off = lpr; off < 64; off <<= 1)
+#pragma unroll
+        for (int i = 0; i < V; i++) {
+            lo[i] = fminf(lo[i], __shfl_xor(lo[i], (int)off));
+            hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], (int)off));
+        }
+    if constexpr (WPU > 1) {
+#pragma unroll
+        for (int i = 0; i < V; i++) { red[w][0][i][lane] = lo[i]; red[w][1][i][lane] = hi[i]; }
+        __syncthreads();
+        if (w) return;
+#pragma unroll
+        for (int i = 0; i < V; i++)
+            for (int k = 1; k < 4; k++) {
+                lo[i] = fminf(lo[i], red[k][0][i][lane]);
+                hi[i] = fmaxf(hi[i], red[k][1][i][lane]);
+            }
+    }
+    float amax = 0.0f;
+#pragma unroll
+    for (int i = 0; i < V; i++) {
+        if (lo[i] > hi[i]) lo[i] = hi[i] = 0.0f;                      // nothing but NaN
+        amax = fmaxf(amax, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
+    }
+    for (unsigned off = lpr >> 1; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, (int)off));
+    if (!ok || (unsigned)lane >= lpr) return;
+    const int e = bounds_exponent(amax);
+    uint32_t cl[V / 4], ch[V / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; i++) {
+        cl[i] = ch[i] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float l = floorf(fminf(fmaxf(ldexpf(lo[4 * i + j], -e), -127.0f), 127.0f));
+            const float g = ceilf(fminf(fmaxf(ldexpf(hi[4 * i + j], -e), -127.0f), 127.0f));
+            cl[i] |= ((uint32_t)(int)l & 0xffu) << (8 * j);
+            ch[i] |= ((uint32_t)(int)g & 0xffu) << (8 * j);
+        }
+    }
+    const size_t entry = ((size_t)layer * a.NB + blk) * a.KVH + h;
+    uint8_t *dst = A.bounds + entry * 2 * a.D + sub * V;
+    if constexpr (V == 8) {
+        *(uint2 *)dst = make_uint2(cl[0], cl[1]);
+        *(uint2 *)(dst + a.D) = make_uint2(ch[0], ch[1]);
+    } else {
+        *(uint4 *)dst = make_uint4(cl[0], cl[1], cl[2], cl[3]);
+        *(uint4 *)(dst + a.D) = make_uint4(ch[0], ch[1], ch[2], ch[3]);
+    }
+    if (sub == 0) A.bounds[A.exps + entry] = (uint8_t)(int8_t)e;
+}
+
+// 16 codes per thread -> 16 bf16 values (7 bits and a power of two: exact)
+__global__ __launch_bounds__(kBThreads) void bounds_extract_kernel(Lay a, uint8_t *__restrict__ dst, const uint8_t *__restrict__ bounds,
+                                                                  size_t exps, const int32_t *__restrict__ blocks, int n_blocks,
+                                                                  int layer0, size_t chunks, int cps)
+{
+    const size_t i = (size_t)blockIdx.x * kBThreads + threadIdx.x;
+    if (i >= chunks) return;
+    const size_t row = i >> cps;                                     // (layer, block, head)
+    const unsigned c = (unsigned)(i & ((1u << cps) - 1));
+    const unsigned h = (unsigned)(row % a.KVH);
+    const size_t lb = row / a.KVH;
+    const int layer = layer0 + (int)(lb / n_blocks), blk = blocks[lb % n_blocks];
+    uint4 o[2] = {};
+    if (blk >= 0 && blk < a.NB) {
+        const size_t entry = ((size_t)layer * a.NB + blk) * a.KVH + h;
+        const uint4 v = *(const uint4 *)(bounds + entry * 2 * a.D + c * 16);
+        const float s = ldexpf(1.0f, (int)(int8_t)bounds[exps + entry]);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        uint32_t y[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float x0 = (float)(int8_t)(w[k / 2] >> (16 * (k & 1))) * s, x1 = (float)(int8_t)(w[k / 2] >> (16 * (k & 1) + 8)) * s;
+            y[k] = (__float_as_uint(x0) >> 16) | (__float_as_uint(x1) & 0xffff0000u);
+        }
+        o[0] = make_uint4(y[0], y[1], y[2], y[3]);
+        o[1] = make_uint4(y[4], y[5], y[6], y[7]);
+    }
+    *(uint4 *)(dst + i * 32) = o[0];
+    *(uint4 *)(dst + i * 32 + 16) = o[1];
+}
+
+int bounds_lay(const drk_kv_layout *g, Lay *a, const char *who)
+{
+    int rc = make_lay(g, a);
+    if (rc) return rc;
+    if (a->D < 64 || a->D > 512 || ilog2_exact((unsigned)a->D) < 0)
+        return fail(DRK_ERR_UNSUPPORTED, "%s: head_dim %d is not a power of two in [64, 512]", who, a->D);
+    return DRK_OK;
+}
+
+} // namespace drk
+
+using namespace drk;
+
+extern "C" {
+
+size_t drk_kv_bounds_bytes(const drk_kv_layout *g)
+{
+    Lay a;
+    if (bounds_lay(g, &a, "kv_bounds_bytes")) return 0;
+    return (bounds_exps_offset(a) + (size_t)a.L * a.NB * a.KVH + 15) & ~(size_t)15;
+}
+
+int drk_kv_bounds_update(const drk_kv_layout *g, const void *pool, const int32_t *d_tables, int table_stride, const int32_t *d_pos,
+                         int pos_start, int n, int layer, int layer_count, void *bounds, void *stream)
+{
+    Lay a;
+    int rc = bounds_lay(g, &a, "kv_bounds_update");
+    if (rc) return rc;
+    if (n < 0 || pos_start < 0 || table_stride < 0 || pos_start > 0x7fffffff - n)
+        return fail(DRK_ERR_INVALID, "kv_bounds_update: bad argument");
+    if (layer < 0 || layer_count < 0 || layer_count > a.L - layer)
+        return fail(DRK_ERR_INVALID, "kv_bounds_update: layers [%d, +%d) outside [0,%d)", layer, layer_count, a.L);
+    if (n == 0 || layer_count == 0) return DRK_OK;
+    if (!pool || !d_tables || !bounds) return fail(DRK_ERR_INVALID, "kv_bounds_update: NULL pointer");
+    if (((uintptr_t)pool | (uintptr_t)bounds) & 15u) return fail(DRK_ERR_INVALID, "kv_bounds_update: pool and bounds must be 16-byte aligned");
+    BoundsArgs A;
+    A.pool = (const uint8_t *)pool; A.bounds = (uint8_t *)bounds; A.tables = d_tables; A.d_pos = d_pos;
+    A.exps = bounds_exps_offset(a);
+    A.table_stride = table_stride; A.pos_start = pos_start; A.n = n; A.layer0 = layer;
+    A.bs_div = mk_div((unsigned)a.bs);
+    A.first_block = d_pos ? 0 : pos_start / a.bs;
+    A.n_blocks = d_pos ? n : (pos_start + n - 1) / a.bs - A.first_block + 1;
+    const size_t units = (size_t)A.n_blocks * a.KVH * layer_count;
+    if (units > 0x7fffffffu) return fail(DRK_ERR_INVALID, "kv_bounds_update: too many blocks");
+    A.units = (unsigned)units;
+    const unsigned lpr = a.row_bytes / 16;
+    const bool wide = (size_t)a.head_stride > 8192;
+    const dim3 grid(wide ? (unsigned)units : (unsigned)((units + 3) / 4));
+    hipStream_t st = (hipStream_t)stream;
+#define DRK_BOUNDS_LAUNCH(DT)                                                                                                     \
+    do {                                                                                                                          \
+        if (wide) hipLaunchKernelGGL((bounds_update_kernel<DT, 4>), grid, dim3(kBThreads), 0, st, a, A, lpr);                     \
+        else hipLaunchKernelGGL((bounds_update_kernel<DT, 1>), grid, dim3(kBThreads), 0, st, a, A, lpr);                          \
+    } while (0)
+    switch (a.dtype) {
+    case DRK_F16: DRK_BOUNDS_LAUNCH(DRK_F16); break;
+    case DRK_BF16: DRK_BOUNDS_LAUNCH(DRK_BF16); break;
+    case DRK_INT8: DRK_BOUNDS_LAUNCH(DRK_INT8); break;
+    default: DRK_BOUNDS_LAUNCH(DRK_FP8_E4M3); break;
+    }
+#undef DRK_BOUNDS_LAUNCH
+    DRK_LAUNCH_CHECK("bounds_update_kernel");
+    return DRK_OK;
+}
+
+int drk_kv_bounds_extract(const drk_kv_layout *g, void *d_dst, const void *bounds, const int32_t *d_blocks, int n_blocks, int layer,
+                          int layer_count, void *stream)
+{
+    Lay a;
+    int rc = bounds_lay(g, &a, "kv_bounds_extract");
+    if (rc) return rc;
+    if (n_blocks < 0) return fail(DRK_ERR_INVALID, "kv_bounds_extract: bad argument");
+    if (layer < 0 || layer_count < 0 || layer_count > a.L - layer)
+        return fail(DRK_ERR_INVALID, "kv_bounds_extract: layers [%d, +%d) outside [0,%d)", layer, layer_count, a.L);
+    if (n_blocks == 0 || layer_count == 0) return DRK_OK;
+    if (!d_dst || !bounds || !d_blocks) return fail(DRK_ERR_INVALID, "kv_bounds_extract: NULL pointer");
+    if (((uintptr_t)d_dst | (uintptr_t)bounds) & 15u) return fail(DRK_ERR_INVALID, "kv_bounds_extract: d_dst and bounds must be 16-byte aligned");
+    const int cps = ilog2_exact((unsigned)a.D / 8);                  // 16-code chunks of a (low, high) pair
+    const size_t chunks = ((size_t)layer_count * n_blocks * a.KVH) << cps, blocks = (chunks + kBThreads - 1) / kBThreads;
+    if (blocks > 0x7fffffffu) return fail(DRK_ERR_INVALID, "kv_bounds_extract: too many blocks");
+    hipLaunchKernelGGL(bounds_extract_kernel, dim3((unsigned)blocks), dim3(kBThreads), 0, (hipStream_t)stream, a, (uint8_t *)d_dst,
+                       (const uint8_t *)bounds, bounds_exps_offset(a), d_blocks, n_blocks, layer, chunks, cps);
+    DRK_LAUNCH_CHECK("bounds_extract_kernel");
+    return DRK_OK;
+}
+
+} // extern "C"

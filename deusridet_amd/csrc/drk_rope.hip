@@ -1,0 +1,218 @@
+// drk_rope.hip -- rotary positions for long contexts: frequencies stretched per pair, either
+// pair layout, part of a head, strided rows, both directions.
+//
+// For a pair (a, b) of a head at position p, with f its turns per position and m the magnitude:
+//   a' = m (a cos w - b sin w),  b' = m (b cos w + a sin w),  w = 2 pi p f
+// (inverse: sin w with the other sign -- the transpose, which is the gradient).  p f is formed in
+// 64 bits and only its fraction of a turn goes on in 32 bits: in 32 bits the angle of position
+// 10^6 would carry an error of 0.06 rad.  The hardware's sine and cosine take turns, so no range
+// reduction follows; their error, about 2^-20, is far below the 16-bit result's rounding.
+#include "drk_common.hpp"
+#include "drk_codec.hpp"
+
+#include <math.h>
+
+namespace drk {
+
+constexpr int kRThreads = 256;
+
+// f'_i, see drk_rope in drk_kv.h
+__device__ __forceinline__ double rope_turns(const drk_rope &r, int i)
+{
+    const double f = pow((double)r.theta, -2.0 * i / r.rotary_dim) * 0.15915494309189533577;   // 1 / (2 pi)
+    if (r.factor == 1.0f) return f;
+    double g = (f * r.original_positions - r.low_turns) / ((double)r.high_turns - r.low_turns);
+    g = g < 0.0 ? 0.0 : (g > 1.0 ? 1.0 : g);
+    return f * (g + (1.0 - g) / r.factor);
+}
+
+// cos and sin of p f turns
+__device__ __forceinline__ void rope_cos_sin(double p, double f, float &c, float &s)
+{
+    const double w = p * f;
+    const float x = (float)(w - floor(w));
+#if defined(__HIP_DEVICE_COMPILE__)
+    c = __builtin_amdgcn_cosf(x);
+    s = __builtin_amdgcn_sinf(x);
+#else
+    c = x;
+    s = x;
+#endif
+}
+
+__global__ __launch_bounds__(kRThreads) void rope_freqs_kernel(drk_rope r, double *__restrict__ freqs)
+{
+    const int i = blockIdx.x * kRThreads + threadIdx.x;
+    if (i < r.rotary_dim / 2) freqs[i] = rope_turns(r, i);
+}
+
+__global__ __launch_bounds__(kRThreads) void rope_table_scaled_kernel(drk_rope r, float *__restrict__ table, int n_pos)
+{
+    const int np = r.rotary_dim / 2;
+    const size_t i = (size_t)blockIdx.x * kRThreads + threadIdx.x;
+    if (i >= (size_t)n_pos * np) return;
+    const int pos = (int)(i / np), pair = (int)(i - (size_t)pos * np);
+    const double w = pos * rope_turns(r, pair);
+    const double x = (w - floor(w)) * 6.28318530717958647693;
+    *(float2 *)(table + i * 2) = make_float2((float)(cos(x) * r.magnitude), (float)(sin(x) * r.magnitude));
+}
+
+struct RopeArgs {
+    drk_rope_rows tensors[DRK_ROPE_MAX_TENSORS];
+    const double *freqs;
+    const int32_t *d_pos;
+    int first_head[DRK_ROPE_MAX_TENSORS];   // head rows before tensor i in a token's list of them
+    int n_tensors, pos_start, T, rows, units, hp, interleaved, dtype;
+    float cm, sm;                           // factors of cos and sin: the magnitude, and its sign turned for the inverse
+};
+
+__device__ __forceinline__ uint4 rope_pack8(const float *y, int dtype)
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        w[i] = (uint32_t)f_to_elem16(y[2 * i], dtype) | ((uint32_t)f_to_elem16(y[2 * i + 1], dtype) << 16);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// One thread: 8 pairs (or 16 elements that pass unchanged) of one head row.
+__global__ __launch_bounds__(kRThreads) void rope_apply_kernel(RopeArgs A)
+{
+    const size_t it = (size_t)blockIdx.x * kRThreads + threadIdx.x;
+    if (it >= (size_t)A.T * A.rows * A.units) return;
+    const size_t row = it / A.units;
+    const int u = (int)(it - row * A.units);
+    const int t = (int)(row / A.rows);
+    int h = (int)(row - (size_t)t * A.rows), n = 0;
+    while (n + 1 < A.n_tensors && h >= A.first_head[n + 1]) n++;
+    h -= A.first_head[n];
+    const drk_rope_rows &R = A.tensors[n];
+    const uint16_t *x = (const uint16_t *)R.x + (size_t)t * R.x_token_stride + (size_t)h * R.x_head_stride;
+    uint16_t *o = (uint16_t *)R.out + (size_t)t * R.out_token_stride + (size_t)h * R.out_head_stride;
+    if (u >= A.hp) {                                   // behind the rotary part
+        const uint4 v0 = *(const uint4 *)(x + u * 16), v1 = *(const uint4 *)(x + u * 16 + 8);
+        *(uint4 *)(o + u * 16) = v0;
+        *(uint4 *)(o + u * 16 + 8) = v1;
+        return;
+    }
+    // half-half: pair (i, i + r/2), so 8 pairs are chunks u and u + hp of 8; interleaved: 16 consecutive elements
+    const int e0 = A.interleaved ? u * 16 : u * 8, e1 = A.interleaved ? e0 + 8 : e0 + A.hp * 8;
+    float a[8], b[8], y0[8], y1[8];
+    unpack8(*(const uint4 *)(x + e0), A.dtype, a);
+    unpack8(*(const uint4 *)(x + e1), A.dtype, b);
+    const double p = A.d_pos ? A.d_pos[t] : (double)A.pos_start + t;
+    float c[8], s[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        rope_cos_sin(p, A.freqs[u * 8 + i], c[i], s[i]);
+        c[i] *= A.cm;
+        s[i] *= A.sm;
+    }
+    if (A.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            y0[2 * i] = a[2 * i] * c[i] - a[2 * i + 1] * s[i];
+            y0[2 * i + 1] = a[2 * i + 1] * c[i] + a[2 * i] * s[i];
+            y1[2 * i] = b[2 * i] * c[i + 4] - b[2 * i + 1] * s[i + 4];
+            y1[2 * i + 1] = b[2 * i + 1] * c[i + 4] + b[2 * i] * s[i + 4];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            y0[i] = a[i] * c[i] - b[i] * s[i];
+            y1[i] = b[i] * c[i] + a[i] * s[i];
+        }
+    }
+    *(uint4 *)(o + e0) = rope_pack8(y0, A.dtype);
+    *(uint4 *)(o + e1) = rope_pack8(y1, A.dtype);
+}
+
+static int check_rope(const drk_rope *r, const char *who)
+{
+    if (!r) return fail(DRK_ERR_INVALID, "%s: NULL description", who);
+    if (r->rotary_dim < 16 || (r->rotary_dim % 16))
+        return fail(DRK_ERR_UNSUPPORTED, "%s: rotary_dim %d must be a multiple of 16", who, r->rotary_dim);
+    if (r->interleaved != 0 && r->interleaved != 1) return fail(DRK_ERR_INVALID, "%s: interleaved must be 0 or 1", who);
+    if (!(r->theta > 0.0f) || !isfinite(r->theta) || !(r->factor > 0.0f) || !isfinite(r->factor) || !isfinite(r->magnitude))
+        return fail(DRK_ERR_INVALID, "%s: theta and factor must be positive, magnitude finite", who);
+    if (r->factor != 1.0f && !(r->original_positions >= 0.0f && r->low_turns >= 0.0f && r->high_turns > r->low_turns &&
+                               isfinite(r->original_positions) && isfinite(r->high_turns)))
+        return fail(DRK_ERR_INVALID, "%s: original_positions >= 0 and 0 <= low_turns < high_turns are wanted", who);
+    return DRK_OK;
+}
+
+} // namespace drk
+
+using namespace drk;
+
+extern "C" {
+
+int drk_rope_freqs_fill(const drk_rope *r, double *d_freqs, void *stream)
+{
+    int rc = check_rope(r, "rope_freqs_fill");
+    if (rc) return rc;
+    if (!d_freqs) return fail(DRK_ERR_INVALID, "rope_freqs_fill: NULL pointer");
+    hipLaunchKernelGGL(rope_freqs_kernel, dim3((r->rotary_dim / 2 + kRThreads - 1) / kRThreads), dim3(kRThreads), 0,
+                       (hipStream_t)stream, *r, d_freqs);
+    DRK_LAUNCH_CHECK("rope_freqs_kernel");
+    return DRK_OK;
+}
+
+int drk_rope_table_fill_scaled(const drk_rope *r, float *d_table, int n_pos, void *stream)
+{
+    int rc = check_rope(r, "rope_table_fill_scaled");
+    if (rc) return rc;
+    if (!d_table || n_pos < 1) return fail(DRK_ERR_INVALID, "rope_table_fill_scaled: bad argument");
+    if (r->interleaved) return fail(DRK_ERR_UNSUPPORTED, "rope_table_fill_scaled: the entry points that read a table rotate half-half pairs");
+    const size_t blocks = ((size_t)n_pos * (r->rotary_dim / 2) + kRThreads - 1) / kRThreads;
+    if (blocks > 0x7fffffffu) return fail(DRK_ERR_INVALID, "rope_table_fill_scaled: table too large");
+    hipLaunchKernelGGL(rope_table_scaled_kernel, dim3((unsigned)blocks), dim3(kRThreads), 0, (hipStream_t)stream, *r, d_table, n_pos);
+    DRK_LAUNCH_CHECK("rope_table_scaled_kernel");
+    return DRK_OK;
+}
+
+int drk_rope_apply(const drk_rope *r, const double *d_freqs, const drk_rope_rows *tensors, int n_tensors, int T, int head_dim,
+                   const int32_t *d_pos, int pos_start, int inverse, int dtype, void *stream)
+{
+    int rc = check_rope(r, "rope_apply");
+    if (rc) return rc;
+    if (dtype != DRK_F16 && dtype != DRK_BF16) return fail(DRK_ERR_INVALID, "rope_apply: dtype must be F16 or BF16");
+    if (head_dim < 16 || head_dim > 1024 || (head_dim % 16) || r->rotary_dim > head_dim)
+        return fail(DRK_ERR_UNSUPPORTED, "rope_apply: head_dim %d must be a multiple of 16 up to 1024, rotary_dim %d at most that",
+                    head_dim, r->rotary_dim);
+    if (!d_freqs || !tensors || n_tensors < 1 || n_tensors > DRK_ROPE_MAX_TENSORS || T < 0 || pos_start < 0)
+        return fail(DRK_ERR_INVALID, "rope_apply: bad argument");
+    RopeArgs A;
+    A.rows = 0;
+    bool in_place = true;
+    for (int i = 0; i < n_tensors; i++) {
+        const drk_rope_rows &x = tensors[i];
+        if (x.heads < 0 || x.reserved != 0 || (x.heads > 0 && T > 0 && (!x.x || !x.out)))
+            return fail(DRK_ERR_INVALID, "rope_apply: tensor %d: bad argument", i);
+        if (((uintptr_t)x.x | (uintptr_t)x.out) & 15u || (x.x_token_stride | x.x_head_stride | x.out_token_stride | x.out_head_stride) & 7u)
+            return fail(DRK_ERR_INVALID, "rope_apply: tensor %d: pointers must be 16-byte aligned, strides multiples of 8", i);
+        if (x.heads > 1 && x.out_head_stride < (size_t)head_dim)
+            return fail(DRK_ERR_INVALID, "rope_apply: tensor %d: heads of out overlap", i);
+        if (x.x == x.out && (x.x_token_stride != x.out_token_stride || x.x_head_stride != x.out_head_stride))
+            return fail(DRK_ERR_INVALID, "rope_apply: tensor %d: in place needs equal strides", i);
+        if (x.heads > (1 << 20)) return fail(DRK_ERR_INVALID, "rope_apply: tensor %d: %d heads", i, x.heads);
+        in_place = in_place && x.x == x.out;
+        A.tensors[i] = x;
+        A.first_head[i] = A.rows;
+        A.rows += x.heads;
+    }
+    A.freqs = d_freqs; A.d_pos = d_pos; A.n_tensors = n_tensors; A.pos_start = pos_start; A.T = T;
+    A.hp = r->rotary_dim / 16;
+    A.units = in_place ? A.hp : head_dim / 16;              // in place, what passes unchanged is there already
+    A.interleaved = r->interleaved; A.dtype = dtype;
+    A.cm = r->magnitude; A.sm = inverse ? -r->magnitude : r->magnitude;
+    const size_t items = (size_t)T * A.rows * A.units;
+    if (items == 0) return DRK_OK;
+    const size_t blocks = (items + kRThreads - 1) / kRThreads;
+    if (blocks > 0x7fffffffu) return fail(DRK_ERR_INVALID, "rope_apply: too many rows");
+    hipLaunchKernelGGL(rope_apply_kernel, dim3((unsigned)blocks), dim3(kRThreads), 0, (hipStream_t)stream, A);
+    DRK_LAUNCH_CHECK("rope_apply_kernel");
+    return DRK_OK;
+}
+
+} // extern "C"

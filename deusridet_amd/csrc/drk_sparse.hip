@@ -1,0 +1,449 @@
+// drk_sparse.hip -- paged GQA attention over the blocks a selection lists for each (row, kv head).
+//
+// The listed blocks' tokens are one long axis, cut into groups of 16 (a block is a whole number of
+// them).  A workgroup takes a piece of one (row, kv head)'s groups: first every thread turns a few
+// groups into descriptors in LDS -- list entry, block table, page offset: the dependent loads happen
+// there, side by side, and groups without a token drop out -- then its four waves walk them
+// independently, each with a running maximum and sum per query head and the output in registers:
+//   S[token][head] = K[16 x D] Q^T       D/32 x v_mfma_f32_16x16x32
+//   O[head][dim]  += P[heads x 16] V     D/16 x v_mfma_f32_16x16x16
+// with the query heads of the group as the 16-wide operand.  The waves' states meet at the end; a row
+// that was cut leaves (o, m, l) per piece for sparse_merge_kernel, otherwise it is written at once.
+#include "drk_stream_tile.hpp"
+
+namespace drk {
+
+constexpr int kSpGroups = 512;          // 16-token groups one workgroup may own (descriptors in LDS)
+constexpr int kSpMaxPieces = 64;        // pieces of a row: a lane each in the merge
+constexpr int kSpWgs = 512;             // workgroups a launch aims at: 2 per CU
+
+struct SparseArgs {
+    const uint8_t *pool_layer, *q;
+    const int32_t *tables, *seq_lens, *sel;
+    const uint16_t *gate;
+    uint16_t *out;
+    float *part_o, *part_m, *part_l;     // [T][QH][pieces]([D])
+    size_t gate_stride;
+    int table_stride, pos_start, KVH, QH, NB, bs, keep, io_dtype;
+    int pieces, groups_per_piece, groups;    // 16-token groups of a (row, kv head)'s list
+    unsigned head_stride, kv_plane, block_stride, scale_plane, row_bytes;
+    float scale_log2e;
+};
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, D == 128 ? 4 : 2) void sparse_kernel(SparseArgs A)
+{
+    using Geo = StreamGeo<DT, D>;
+    [[maybe_unused]] constexpr bool Q8 = Geo::q8;
+    constexpr int DOT = KvTraits<DT>::dot;
+    __shared__ __align__(16) uint8_t k_lds[4][16 * Geo::PITCH];
+    __shared__ __align__(16) float o_lds[4][4][D];
+    __shared__ float mw_lds[4][16], lw_lds[4][16];
+    __shared__ uint32_t goff[kSpGroups], gsoff[DT == DRK_INT8 ? kSpGroups : 1];
+    __shared__ uint8_t gcnt[kSpGroups];
+    __shared__ int wcount[4];
+
+    const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int GQ = A.QH / A.KVH;
+    // kv heads vary fastest: neighbouring workgroups, on different XCDs, read different heads' rows
+    const int h = (int)(blockIdx.x % (unsigned)A.KVH), tp = (int)(blockIdx.x / (unsigned)A.KVH);
+    const int t = tp / A.pieces, piece = tp - t * A.pieces;
+    const int len = A.seq_lens ? A.seq_lens[t] : A.pos_start + t + 1;
+    const int bq = t * A.QH + h * GQ;
+
+    // ---- descriptors of the groups that hold tokens, in order ----
+    const int32_t *sel = A.sel + ((size_t)t * A.KVH + h) * A.keep;
+    const int32_t *tab = A.tables + (size_t)t * A.table_stride;
+    const int g0 = piece * A.groups_per_piece, gn = min(A.groups_per_piece, A.groups - g0), gpb = A.bs / 16;
+    int n = 0;
+    for (int i0 = 0; i0 < gn; i0 += 256) {
+        const int gi = g0 + i0 + (int)threadIdx.x;
+        uint32_t off = 0, soff = 0;
+        int cnt = 0;
+        if (i0 + (int)threadIdx.x < gn) {
+            const int e = gi / gpb, lb = sel[e], p0 = (gi - e * gpb) * 16;
+            if (lb >= 0 && lb <= (len - 1) / A.bs && len > 0) {
+                cnt = min(16, len - lb * A.bs - p0);
+                if (cnt > 0) {
+                    const int blk = tab[lb];
+                    if (blk >= 0 && blk < A.NB) {
+                        const size_t base = (size_t)blk * A.block_stride;
+                        off = (uint32_t)((base + (size_t)h * A.head_stride + (size_t)p0 * A.row_bytes) >> 4);
+                        soff = (uint32_t)((base + 2 * (size_t)A.kv_plane + ((size_t)h * A.bs + p0) * 2) >> 4);
+                    } else {
+                        cnt = 0;
+                    }
+                }
+            }
+        }
+        const uint64_t live = __ballot(cnt > 0);
+        if (lane == 0) wcount[w] = __popcll(live);
+        __syncthreads();
+        int at = n + __popcll(live & ((1ull << lane) - 1));
+        for (int i = 0; i < 4; i++) {
+            if (i < w) at += wcount[i];
+            n += wcount[i];
+        }
+        if (cnt > 0) {
+            goff[at] = off;
+            gcnt[at] = (uint8_t)cnt;
+            if (DT == DRK_INT8) gsoff[at] = soff;
+        }
+        __syncthreads();
+    }
+
+    // ---- Q^T as the second operand: lane (head c, dims 32 kk + 8 g ..), heads GQ..15 are padding ----
+    uint4 qop[Geo::NQK];
+    float qbias = 0.0f;
+    {
+        float sq = 0.0f;
+#pragma unroll
+        for (int kk = 0; kk < Geo::NQK; kk++) {
+            uint4 v = make_uint4(0u, 0u, 0u, 0u);
+            if (c < GQ) v = *(const uint4 *)(A.q + (size_t)(bq + c) * (D * 2) + kk * 64 + g * 16);
+#if defined(__HIP_DEVICE_COMPILE__)
+            if (Q8 && A.io_dtype == DRK_BF16) {              // quantised pages multiply in fp16
+                v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.x), bf16_hi(v.x)));
+                v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.y), bf16_hi(v.y)));
+                v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.z), bf16_hi(v.z)));
+                v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.w), bf16_hi(v.w)));
+            }
+#endif
+            qop[kk] = v;
+            if (DT == DRK_INT8) {
+                sq = s_dot2<DOT>(v.x, kF16Ones, sq);
+                sq = s_dot2<DOT>(v.y, kF16Ones, sq);
+                sq = s_dot2<DOT>(v.z, kF16Ones, sq);
+                sq = s_dot2<DOT>(v.w, kF16Ones, sq);
+            }
+        }
+        if (DT == DRK_INT8) {
+            sq += __shfl_xor(sq, 16);
+            sq += __shfl_xor(sq, 32);
+            qbias = kI8Bias * sq;
+        }
+    }
+
+    w_f32x4 o[Geo::NPV];
+#pragma unroll
+    for (int e = 0; e < Geo::NPV; e++) o[e] = w_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float m_run = -INFINITY, l_lane = 0.0f, ps_lane = 0.0f;
+    uint8_t *const klds = &k_lds[w][0];
+    auto load_scales = [&](int i, uint2 &ks, uint2 &vs) {
+        if (DT != DRK_INT8) return;
+        const uint8_t *p = A.pool_layer + ((size_t)gsoff[DT == DRK_INT8 ? i : 0] << 4) + g * 8;
+        ks = *(const uint2 *)p;
+        vs = *(const uint2 *)(p + A.scale_plane);
+    };
+
+    KRegs<DT, D> kreg = {};
+    VRegs<DT, D> vreg = {};
+    uint2 ksr = {}, vsr = {};
+    if (w < n) {
+        kreg = load_k<DT, D>(A.pool_layer, goff[w], lane);
+        vreg = load_v<DT, D>(A.pool_layer, goff[w], A.kv_plane, lane);
+        load_scales(w, ksr, vsr);
+    }
+    for (int i = w; i < n; i += 4) {
+        const int lim = __builtin_amdgcn_readfirstlane((int)gcnt[i]);
+        const bool more = i + 4 < n;
+        stage_k<DT, D>(klds, kreg, lane);
+        float ks[4] = {1.0f, 1.0f, 1.0f, 1.0f}, vs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+        if (DT == DRK_INT8) {
+            ks[0] = f16_bits_to_f((uint16_t)(ksr.x & 0xffffu)); ks[1] = f16_bits_to_f((uint16_t)(ksr.x >> 16));
+            ks[2] = f16_bits_to_f((uint16_t)(ksr.y & 0xffffu)); ks[3] = f16_bits_to_f((uint16_t)(ksr.y >> 16));
+            vs[0] = f16_bits_to_f((uint16_t)(vsr.x & 0xffffu)); vs[1] = f16_bits_to_f((uint16_t)(vsr.x >> 16));
+            vs[2] = f16_bits_to_f((uint16_t)(vsr.y & 0xffffu)); vs[3] = f16_bits_to_f((uint16_t)(vsr.y >> 16));
+        }
+        uint32_t next = 0;
+        if (more) {
+            next = goff[i + 4];
+            kreg = load_k<DT, D>(A.pool_layer, next, lane);
+            load_scales(i + 4, ksr, vsr);
+        }
+        w_f32x4 sacc = {0.0f, 0.0f, 0.0f, 0.0f};
+        const uint8_t *arow = klds + c * Geo::PITCH + g * 16;
+#pragma unroll
+        for (int k0 = 0; k0 < Geo::NQK; k0 += 4) {
+            uint4 ka[4];
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) ka[kk] = *(const uint4 *)(arow + (k0 + kk) * 64);
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) sacc = w_mfma_qk<DOT>(ka[kk], qop[k0 + kk], sacc);
+        }
+        // softmax of head c over tokens 4g..4g+3 (+ the other three lane groups)
+        const int t0 = g * 4;
+        float sc[4], p[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float x = sacc[j];
+            if (DT == DRK_INT8) x = (x - qbias) * ks[j];
+            x *= A.scale_log2e;
+            sc[j] = t0 + j < lim ? x : -INFINITY;
+        }
+        float mloc = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
+        mloc = fmaxf(mloc, __shfl_xor(mloc, 32));
+        const float m_new = fmaxf(m_run, mloc), m_use = m_new == -INFINITY ? 0.0f : m_new;
+        const float alpha = s_exp2(m_run - m_use);
+        m_run = m_new;
+        float pw[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            p[j] = s_exp2(sc[j] - m_use);
+            pw[j] = DT == DRK_INT8 ? (t0 + j < lim ? p[j] * vs[j] : 0.0f) : p[j];
+        }
+        uint2 pa;                                             // P[head c][tokens 4g..4g+3] for the second product
+        if constexpr (DOT == DRK_BF16) {
+            pa.x = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)pw[0]) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)pw[1]) << 16);
+            pa.y = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)pw[2]) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)pw[3]) << 16);
+        } else {
+            pa.x = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)pw[0]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)pw[1]) << 16);
+            pa.y = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)pw[2]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)pw[3]) << 16);
+        }
+        // the denominator sums the rounded weights the product multiplies, so both carry the same rounding
+        // (int8: the product multiplies p times the V scale; its own sum takes the code offset out again)
+        float rs;
+        if (DT == DRK_INT8) {
+            float tsum = s_dot2<DOT>(pa.x, kF16Ones, 0.0f);
+            tsum = s_dot2<DOT>(pa.y, kF16Ones, tsum);
+            ps_lane = fmaf(ps_lane, alpha, tsum);
+            rs = (p[0] + p[1]) + (p[2] + p[3]);
+        } else {
+            const uint32_t ones = DOT == DRK_BF16 ? kBf16Ones : kF16Ones;
+            rs = s_dot2<DOT>(pa.y, ones, s_dot2<DOT>(pa.x, ones, 0.0f));
+        }
+        l_lane = fmaf(l_lane, alpha, rs);
+        if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+            const float a0 = __shfl(alpha, 4 * g), a1 = __shfl(alpha, 4 * g + 1);
+            const float a2 = __shfl(alpha, 4 * g + 2), a3 = __shfl(alpha, 4 * g + 3);
+#pragma unroll
+            for (int e = 0; e < Geo::NPV; e++) { o[e][0] *= a0; o[e][1] *= a1; o[e][2] *= a2; o[e][3] *= a3; }
+        }
+        if (DT != DRK_INT8 && lim < 16) {                     // rows without a token may hold anything (NaN)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (t0 + j >= lim) {
+#pragma unroll
+                    for (int ch = 0; ch < Geo::NCH; ch++) vreg.r[j][ch] = {};
+                }
+        }
+#pragma unroll
+        for (int ch = 0; ch < Geo::NCH; ch++) {
+            uint2 vb[8];
+            v_operands<DT>(vreg.r[0][ch], vreg.r[1][ch], vreg.r[2][ch], vreg.r[3][ch], vb);
+#pragma unroll
+            for (int e = 0; e < 8; e++) o[ch * 8 + e] = w_mfma_pv<DOT>(pa, vb[e], o[ch * 8 + e]);
+        }
+        if (more) vreg = load_v<DT, D>(A.pool_layer, next, A.kv_plane, lane);
+    }
+
+    // ---- fold the four waves ----
+    float lw = l_lane, psum = ps_lane;
+    lw += __shfl_xor(lw, 16);
+    lw += __shfl_xor(lw, 32);
+    if (DT == DRK_INT8) {
+        psum += __shfl_xor(psum, 16);
+        psum += __shfl_xor(psum, 32);
+    }
+    if (lane < 16) { mw_lds[w][lane] = m_run; lw_lds[w][lane] = lw; }
+    __syncthreads();
+    float f_own[4], bias[4];                                  // this wave's weight / code offset for head 4g + j
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int hh = 4 * g + j;
+        const float M = fmaxf(fmaxf(mw_lds[0][hh], mw_lds[1][hh]), fmaxf(mw_lds[2][hh], mw_lds[3][hh]));
+        const float mo = mw_lds[w][hh];
+        f_own[j] = mo == -INFINITY ? 0.0f : s_exp2(mo - M);
+        bias[j] = DT == DRK_INT8 ? kI8Bias * __shfl(psum, hh) : 0.0f;
+    }
+    for (int r = 0; r < (GQ + 3) >> 2; r++) {                 // 4 heads per round: head 4r + w is stored by wave w
+        if (r > 0) __syncthreads();
+        if (g == r) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+#pragma unroll
+                for (int ch = 0; ch < Geo::NCH; ch++) {
+                    float *dst = &o_lds[w][j][ch * 128 + c * 8];
+                    const w_f32x4 *oc = &o[ch * 8];
+                    *(float4 *)dst = make_float4((oc[0][j] - bias[j]) * f_own[j], (oc[1][j] - bias[j]) * f_own[j],
+                                                 (oc[2][j] - bias[j]) * f_own[j], (oc[3][j] - bias[j]) * f_own[j]);
+                    *(float4 *)(dst + 4) = make_float4((oc[4][j] - bias[j]) * f_own[j], (oc[5][j] - bias[j]) * f_own[j],
+                                                       (oc[6][j] - bias[j]) * f_own[j], (oc[7][j] - bias[j]) * f_own[j]);
+                }
+        }
+        __syncthreads();
+        const int hh = 4 * r + w;
+        if (hh >= GQ) continue;
+        const float M = fmaxf(fmaxf(mw_lds[0][hh], mw_lds[1][hh]), fmaxf(mw_lds[2][hh], mw_lds[3][hh]));
+        float L = 0.0f;
+#pragma unroll
+        for (int ww = 0; ww < 4; ww++) {
+            const float ll = lw_lds[ww][hh];
+            if (ll != 0.0f) L = fmaf(ll, s_exp2(mw_lds[ww][hh] - M), L);      // (a NaN takes part)
+        }
+        constexpr int VEC = D / 64;
+        const int d = lane * VEC;
+        float acc[VEC];
+#pragma unroll
+        for (int x = 0; x < VEC; x++) acc[x] = (o_lds[0][w][d + x] + o_lds[1][w][d + x]) + (o_lds[2][w][d + x] + o_lds[3][w][d + x]);
+        if (A.pieces > 1) {
+            const size_t pi = (size_t)(bq + hh) * A.pieces + piece;
+#pragma unroll
+            for (int x = 0; x < VEC; x++) A.part_o[pi * D + d + x] = acc[x];
+            if (lane == 0) { A.part_m[pi] = M; A.part_l[pi] = L; }
+        } else if (L != 0.0f) {
+            uint16_t *dst = A.out + (size_t)(bq + hh) * D + d;
+            const uint16_t *gp = A.gate ? A.gate + (size_t)(bq + hh) * A.gate_stride + d : nullptr;
+#pragma unroll
+            for (int x = 0; x < VEC; x++) {
+                float y = acc[x] / L;
+                if (gp) y = sigmoid_gate_value(y, elem16_to_f(gp[x], A.io_dtype));
+                dst[x] = f_to_elem16(y, A.io_dtype);
+            }
+        }
+    }
+}
+
+// grid T * QH, one wave: lane s owns the weight of piece s
+template <int D>
+__global__ __launch_bounds__(64) void sparse_merge_kernel(SparseArgs A)
+{
+    constexpr int VEC = D / 64;
+    const size_t row = blockIdx.x, base = row * A.pieces;
+    const int lane = threadIdx.x, d = lane * VEC;
+    const bool mine = lane < A.pieces;
+    const float m = mine ? A.part_m[base + lane] : -INFINITY, l = mine ? A.part_l[base + lane] : 0.0f;
+    const bool live = l != 0.0f;                               // (a NaN takes part)
+    const float M = s_wave_max(live ? m : -INFINITY);
+    if (__ballot(live) == 0) return;                           // no token took part
+    const float wgt = live ? s_exp2(m - M) : 0.0f;
+    const float L = s_wave_sum(live ? l * wgt : 0.0f);
+    float acc[VEC] = {};
+    for (int s = 0; s < A.pieces; s++) {
+        const float ws = s_lane(wgt, s);
+#pragma unroll
+        for (int x = 0; x < VEC; x++) acc[x] = fmaf(A.part_o[(base + s) * D + d + x], ws, acc[x]);
+    }
+    uint16_t *dst = A.out + row * D + d;
+    const uint16_t *gp = A.gate ? A.gate + row * A.gate_stride + d : nullptr;
+#pragma unroll
+    for (int x = 0; x < VEC; x++) {
+        float y = acc[x] / L;
+        if (gp) y = sigmoid_gate_value(y, elem16_to_f(gp[x], A.io_dtype));
+        dst[x] = f_to_elem16(y, A.io_dtype);
+    }
+}
+
+// Pieces of a (row, kv head): enough workgroups for the chip, but no piece shorter than four groups (one per wave)
+// and none longer than the descriptor table.
+static int sparse_pieces(const Lay &a, int T, int n_keep, int *groups_per_piece)
+{
+    const size_t groups = (size_t)n_keep * (a.bs / 16), rows = (size_t)T * a.KVH;
+    size_t p = (kSpWgs + rows - 1) / rows;
+    p = p > (groups + 3) / 4 ? (groups + 3) / 4 : p;
+    p = p > kSpMaxPieces ? kSpMaxPieces : p;
+    const size_t least = (groups + kSpGroups - 1) / kSpGroups;
+    p = p < least ? least : p;
+    if (p > kSpMaxPieces) return 0;
+    *groups_per_piece = (int)((groups + p - 1) / p);
+    return (int)((groups + *groups_per_piece - 1) / *groups_per_piece);
+}
+
+static int sparse_check(const drk_kv_layout *g, Lay *a, int T, int n_keep, int *pieces, int *gpp, const char *who)
+{
+    int rc = make_lay(g, a);
+    if (rc) return rc;
+    if ((a->D != 128 && a->D != 256) || (a->bs % 16) || a->QH / a->KVH > 16)
+        return fail(DRK_ERR_UNSUPPORTED, "%s: head_dim 128 or 256, block_size a multiple of 16 and at most 16 query heads per kv "
+                    "head are supported (head_dim %d, block_size %d, %d heads)", who, a->D, a->bs, a->QH / a->KVH);
+    if ((a->layer_stride >> 4) > 0xfffffffeu) return fail(DRK_ERR_UNSUPPORTED, "%s: one layer of the pool exceeds 64 GiB", who);
+    if (T < 0 || n_keep < 1) return fail(DRK_ERR_INVALID, "%s: T %d, n_keep %d", who, T, n_keep);
+    *pieces = *gpp = 1;
+    if (T == 0) return DRK_OK;
+    *pieces = sparse_pieces(*a, T, n_keep, gpp);
+    if (*pieces == 0) return fail(DRK_ERR_UNSUPPORTED, "%s: n_keep %d blocks of %d tokens: at most %d tokens per row", who, n_keep, a->bs,
+                                  kSpMaxPieces * kSpGroups * 16);
+    if ((size_t)T * *pieces * a->KVH > 0x7fffffffu || (size_t)T * a->QH > 0x7fffffffu)
+        return fail(DRK_ERR_UNSUPPORTED, "%s: T %d is more than one launch takes", who, T);
+    return DRK_OK;
+}
+
+static size_t sparse_need(const Lay &a, int T, int pieces)
+{
+    return pieces > 1 ? (size_t)T * a.QH * pieces * (a.D + 2) * 4 : 0;
+}
+
+} // namespace drk
+
+using namespace drk;
+
+extern "C" {
+
+size_t drk_paged_sparse_workspace_bytes(const drk_kv_layout *g, int T, int n_keep)
+{
+    Lay a;
+    int pieces, gpp;
+    if (sparse_check(g, &a, T, n_keep, &pieces, &gpp, "paged_sparse_workspace_bytes")) return 0;
+    return sparse_need(a, T, pieces);
+}
+
+int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void *pool, const int32_t *d_tables, int table_stride,
+                               const int32_t *d_seq_lens, int pos_start, int T, const int32_t *d_selected, int n_keep, void *out,
+                               int layer, float scale, int io_dtype, const void *gate, size_t gate_stride, void *workspace,
+                               size_t workspace_bytes, void *stream)
+{
+    Lay a;
+    SparseArgs A;
+    int rc = sparse_check(g, &a, T, n_keep, &A.pieces, &A.groups_per_piece, "paged_sparse_attention");
+    if (rc) return rc;
+    if (io_dtype != DRK_F16 && io_dtype != DRK_BF16) return fail(DRK_ERR_INVALID, "paged_sparse_attention: io_dtype must be F16 or BF16");
+    if (a.E == 2 && io_dtype != a.dtype)
+        return fail(DRK_ERR_INVALID, "paged_sparse_attention: io_dtype %d differs from the pool's %d", io_dtype, a.dtype);
+    if (layer < 0 || layer >= a.L) return fail(DRK_ERR_INVALID, "paged_sparse_attention: layer %d outside [0,%d)", layer, a.L);
+    if (table_stride < 0 || pos_start < 0 || pos_start > 0x7fffffff - T || !(scale > 0.0f))
+        return fail(DRK_ERR_INVALID, "paged_sparse_attention: bad argument");
+    if (T == 0) return DRK_OK;
+    if (!q || !pool || !d_tables || !d_selected || !out) return fail(DRK_ERR_INVALID, "paged_sparse_attention: NULL pointer");
+    if (((uintptr_t)q | (uintptr_t)pool | (uintptr_t)out | (uintptr_t)workspace | (uintptr_t)gate) & 15u)
+        return fail(DRK_ERR_INVALID, "paged_sparse_attention: q, pool, out, gate and the workspace must be 16-byte aligned");
+    if (gate && (gate_stride < (size_t)a.D || (gate_stride % 8)))
+        return fail(DRK_ERR_INVALID, "paged_sparse_attention: gate_stride %zu must be a multiple of 8, at least head_dim", gate_stride);
+    const size_t need = sparse_need(a, T, A.pieces);
+    if (need && (!workspace || workspace_bytes < need))
+        return fail(DRK_ERR_WORKSPACE, "paged_sparse_attention: %zu bytes of workspace, %zu needed", workspace_bytes, need);
+    A.pool_layer = (const uint8_t *)pool + (size_t)layer * a.layer_stride;
+    A.q = (const uint8_t *)q; A.tables = d_tables; A.seq_lens = d_seq_lens; A.sel = d_selected;
+    A.gate = (const uint16_t *)gate; A.gate_stride = gate_stride; A.out = (uint16_t *)out;
+    const size_t np = (size_t)T * a.QH * A.pieces;
+    A.part_o = (float *)workspace; A.part_m = A.part_o + np * a.D; A.part_l = A.part_m + np;
+    A.table_stride = table_stride; A.pos_start = pos_start; A.KVH = a.KVH; A.QH = a.QH; A.NB = a.NB; A.bs = a.bs;
+    A.keep = n_keep; A.io_dtype = io_dtype; A.groups = n_keep * (a.bs / 16);
+    A.head_stride = a.head_stride; A.kv_plane = a.kv_plane; A.block_stride = a.block_stride; A.scale_plane = a.scale_plane;
+    A.row_bytes = a.row_bytes;
+    A.scale_log2e = scale * kSLog2e;
+    hipStream_t st = (hipStream_t)stream;
+    const dim3 grid((unsigned)((size_t)T * A.pieces * a.KVH));
+#define DRK_SPARSE_LAUNCH(DT)                                                                              \
+    do {                                                                                                   \
+        if (a.D == 128) hipLaunchKernelGGL((sparse_kernel<DT, 128>), grid, dim3(256), 0, st, A);           \
+        else hipLaunchKernelGGL((sparse_kernel<DT, 256>), grid, dim3(256), 0, st, A);                      \
+    } while (0)
+    switch (a.dtype) {
+    case DRK_F16: DRK_SPARSE_LAUNCH(DRK_F16); break;
+    case DRK_BF16: DRK_SPARSE_LAUNCH(DRK_BF16); break;
+    case DRK_INT8: DRK_SPARSE_LAUNCH(DRK_INT8); break;
+    default: DRK_SPARSE_LAUNCH(DRK_FP8_E4M3); break;
+    }
+#undef DRK_SPARSE_LAUNCH
+    DRK_LAUNCH_CHECK("sparse_kernel");
+    if (A.pieces > 1) {
+        if (a.D == 128) hipLaunchKernelGGL((sparse_merge_kernel<128>), dim3(T * a.QH), dim3(64), 0, st, A);
+        else hipLaunchKernelGGL((sparse_merge_kernel<256>), dim3(T * a.QH), dim3(64), 0, st, A);
+        DRK_LAUNCH_CHECK("sparse_merge_kernel");
+    }
+    return DRK_OK;
+}
+
+} // extern "C"

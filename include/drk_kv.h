@@ -469,6 +469,107 @@ int drk_importance_update(float *d_scores, const float *d_new_scores, int n, flo
  * reference counterpart: the reference's scorer is never fed).  One launch, no memset node: may be captured. */
 int drk_importance_fold_clear(float *d_scores, float *d_new_scores, int n, float decay, void *stream);
 
+/* ---- long contexts: stretched rotary positions ---------------------------- */
+/* Rotary embedding with frequencies stretched for contexts longer than the trained one, in either pair layout, over
+ * part of a head (no reference counterpart: its rope is unscaled, half-half, fp32 angles, layer_attention.cu:32-69).
+ * Pair i turns f_i = theta^(-2 i / rotary_dim) / (2 pi) times per position.  A pair that makes high_turns or more
+ * over original_positions keeps its frequency, one that makes low_turns or fewer has it divided by factor, in between
+ * the two are mixed linearly in the turns:
+ *   f'_i = f_i * (g + (1 - g) / factor),  g = clamp((original_positions * f_i - low_turns) / (high_turns - low_turns), 0, 1)
+ * factor 1 leaves every frequency alone (the three numbers are then not read); original_positions 0 stretches every
+ * pair.  cos and sin are multiplied by magnitude (1 = plain rotation). */
+typedef struct drk_rope {
+    int32_t rotary_dim;          /* multiple of 16, at most head_dim; the rest of a head passes unchanged */
+    int32_t interleaved;         /* 0: pairs (i, i + rotary_dim/2); 1: pairs (2i, 2i + 1) */
+    float theta, factor, original_positions, low_turns, high_turns, magnitude;
+} drk_rope;
+/* The frequencies f'_i as double [rotary_dim/2], formed in 64 bits: filled once, read by every drk_rope_apply. */
+int drk_rope_freqs_fill(const drk_rope *r, double *d_freqs, void *stream);
+/* A cos/sin table for the entry points that take one (drk_apply_rope, drk_qk_norm_rope_append: half-half pairs,
+ * rotary_dim = 16 * 2^k there): float [n_pos][rotary_dim/2][2] of magnitude * (cos, sin)(2 pi pos f'_i), the angle in
+ * 64 bits and reduced before it is rounded.  Those entry points evaluate unstretched angles beyond the table: cover
+ * every position. */
+int drk_rope_table_fill_scaled(const drk_rope *r, float *d_table, int n_pos, void *stream);
+/* One tensor of head rows: element (t, head, d) at t * token_stride + head * head_stride + d; strides in elements,
+ * multiples of 8, pointers 16-byte aligned.  out may equal x with the same strides (in place); otherwise the two must
+ * not overlap. */
+typedef struct drk_rope_rows {
+    const void *x;
+    void *out;
+    int32_t heads, reserved;     /* reserved must be 0 */
+    size_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+} drk_rope_rows;
+#define DRK_ROPE_MAX_TENSORS 4
+/* Rotates T tokens of n_tensors tensors (q and k, say) in one launch.  d_pos != NULL: token t is at d_pos[t];
+ * otherwise at pos_start + t.  The angle is formed in 64 bits, so positions of millions keep their accuracy.
+ * inverse != 0 rotates by the negative angle with the same magnitude: the gradient of the call with inverse = 0.
+ * head_dim is a multiple of 16 up to 1024; elements are DRK_F16 or DRK_BF16, arithmetic 32-bit, one rounding. */
+int drk_rope_apply(const drk_rope *r, const double *d_freqs, const drk_rope_rows *tensors, int n_tensors, int T,
+                   int head_dim, const int32_t *d_pos, int pos_start, int inverse, int dtype, void *stream);
+
+/* ---- long contexts: attention over selected blocks -------------------------- */
+/* A decode step over a very long context can read a few blocks of it instead of all (no reference counterpart; the
+ * intent is that of the importance-driven cache, docs/en/architecture/02-memoria.md:40-44).  Three calls: the bounds
+ * of every block's keys are kept beside the pages (drk_kv_bounds_update, after the append); a query scores every block
+ * against its bounds and keeps the best (drk_block_select); attention reads those (drk_paged_sparse_attention).
+ *
+ * Bounds of (layer, physical block, kv head): for every dimension the lowest and the highest key value of the block,
+ * as int8 codes of one power of two, rounded outward:
+ *   e = the smallest whole number in [-40, 40] with max |k| <= 127 * 2^e  (40 if there is none: values beyond are
+ *   taken as +-127 * 2^40),  low = floor(min k / 2^e),  high = ceil(max k / 2^e).
+ * NaN keys are passed over (a dimension that holds nothing else has low = high = 0).
+ * Buffer of drk_kv_bounds_bytes(): codes int8 [layers][blocks][kv heads][2 (low, high)][head_dim], then exponents
+ * int8 [layers][blocks][kv heads]; 16-byte aligned.  It need not be cleared: entries mean something once updated.
+ * head_dim is a power of two in [64, 512], any storage type, any block size. */
+size_t drk_kv_bounds_bytes(const drk_kv_layout *g);
+/* Recomputes, from the pages, the bounds of the blocks that received tokens; layers layer .. layer + layer_count - 1.
+ * d_pos != NULL: one token for each of n branches, at d_pos[i] of table row i -- the block of d_pos[i] is covered up to
+ * d_pos[i] (a negative position or a missing page is skipped).  NULL: tokens [pos_start, pos_start + n) of one table --
+ * their blocks, up to pos_start + n - 1.  Tokens before pos_start in the first block count: the block is recomputed,
+ * not added to, so copies made on write, reused pages and rewritten positions need nothing special.  Two branches
+ * whose positions lie in the same physical block (they must not both write it) leave it covered up to one of them. */
+int drk_kv_bounds_update(const drk_kv_layout *g, const void *pool, const int32_t *d_tables, int table_stride,
+                         const int32_t *d_pos, int pos_start, int n, int layer, int layer_count, void *bounds,
+                         void *stream);
+/* The values the bounds stand for: d_dst bf16 [layer_count][n_blocks][kv heads][2][head_dim] (exact) of the physical
+ * blocks d_blocks[n_blocks] -- a stretch of a block table; a hole (< 0) is zero-filled. */
+int drk_kv_bounds_extract(const drk_kv_layout *g, void *d_dst, const void *bounds, const int32_t *d_blocks, int n_blocks,
+                          int layer, int layer_count, void *stream);
+
+/* For each of T query rows and each kv head: n_keep logical blocks, ascending, -1 behind the last, into
+ * d_selected int32 [T][num_kv_heads][n_keep].  Row t sees seq_len tokens: d_seq_lens[t], or pos_start + t + 1 when
+ * d_seq_lens is NULL; its table row is t * table_stride (0: one table for all rows).  Blocks of the row are
+ * [0, ceil(seq_len / block_size)); those without a page are never selected.  The first n_sink and the last n_recent
+ * blocks are always kept, the others by their score, highest first, equal scores by the lower index.  The score is
+ * the largest over the kv head's query heads of
+ *   2^(eq + e) * sum_d max(c_d * low_d, c_d * high_d),   c_d = rint(q_d / 2^eq),  eq as e above from max |q_d|
+ * -- (up to the rounding of q) an upper bound of every logit the block can give.  It is a whole number below 2^24
+ * times a power of two: exact in 32 bits, the same for any order of summation.  NaN in q counts as 0.
+ * max_seq_len bounds every row's length (a longer one is cut to it) and sizes the workspace, which need not be
+ * cleared: drk_block_select_workspace_bytes, 16-byte aligned.  1 <= n_keep, n_sink + n_recent <= n_keep; at most 16
+ * query heads per kv head; head_dim as for the bounds; io_dtype DRK_F16 / DRK_BF16.  Rows of length <= 0 get -1. */
+size_t drk_block_select_workspace_bytes(const drk_kv_layout *g, int T, int max_seq_len);
+int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, const void *q, int io_dtype,
+                     const int32_t *d_tables, int table_stride, const int32_t *d_seq_lens, int pos_start, int T,
+                     int max_seq_len, int n_keep, int n_sink, int n_recent, int32_t *d_selected, void *workspace,
+                     size_t workspace_bytes, void *stream);
+
+/* GQA attention of T query rows over the blocks listed for each (row, kv head): d_selected [T][num_kv_heads][n_keep]
+ * logical blocks in any order; an entry that is negative, lies behind the row's last token, or has no page is passed
+ * over, one that is listed twice counts twice.  Rows, lengths and tables as in drk_block_select; q / out
+ * [T, num_q_heads, head_dim] of io_dtype; a row sees only its first seq_len tokens.  out = attention, or with a gate
+ * attention * sigmoid(gate) (rows gate_stride elements apart, 16-byte aligned), rounded once; a row without a token,
+ * or whose every score is -inf, is left as it was.  head_dim 128 or 256, block_size % 16 == 0, at most 16 query heads per kv head, every storage
+ * type (as the page's own type when it is 16 bits, io_dtype must equal it); DRK_ERR_UNSUPPORTED otherwise.
+ * One layer of the pool holds at most 64 GiB.  Workspace for the pieces of rows that are cut:
+ * drk_paged_sparse_workspace_bytes, 16-byte aligned, not cleared. */
+size_t drk_paged_sparse_workspace_bytes(const drk_kv_layout *g, int T, int n_keep);
+int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void *pool, const int32_t *d_tables,
+                               int table_stride, const int32_t *d_seq_lens, int pos_start, int T,
+                               const int32_t *d_selected, int n_keep, void *out, int layer, float scale, int io_dtype,
+                               const void *gate, size_t gate_stride, void *workspace, size_t workspace_bytes,
+                               void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,10 +68,7 @@ class RopeRows(C.Structure):
 def rope_rows(tensors):
     """ctypes array of drk_rope_rows from (x, out, heads, x token stride, x head stride, out token stride, out head
     stride) tuples: addresses, and strides in elements"""
-    arr = (RopeRows * len(tensors))()
-    for i, (x, out, heads, *strides) in enumerate(tensors):
-        arr[i] = RopeRows(x, out, heads, 0, *strides)
-    return arr
+    return (RopeRows * len(tensors))(*[(x, out, heads, 0, *strides) for x, out, heads, *strides in tensors])
 
 
 _vp, _i32, _sz, _f32 = C.c_void_p, C.c_int32, C.c_size_t, C.c_float
@@ -277,7 +274,15 @@ def time_partial_kernels(call_one, n, warm=6):
     return sum(e0.elapsed_time(e1) for e0, e1 in ev) / n
 
 
+_current_raw_stream = None
+
+
 def stream_ptr():
     """The hipStream_t of torch's current stream, as the entry points take it."""
-    import torch
-    return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    global _current_raw_stream
+    if _current_raw_stream is None:
+        import torch
+        torch.cuda.init()                  # the two functions below expect an initialised device
+        _current_raw_stream = (torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice)
+    raw, device = _current_raw_stream
+    return C.c_void_p(raw(device()))

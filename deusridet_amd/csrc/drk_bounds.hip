@@ -12,6 +12,7 @@
 namespace drk {
 
 constexpr int kBThreads = 256;
+constexpr int kBLongBlock = 32;            // tokens per block from which a workgroup takes a unit
 
 struct BoundsArgs {
     const uint8_t *pool;
@@ -51,90 +52,99 @@ __device__ __forceinline__ void bounds_unpack(const uint4 &v, float scale, float
     }
 }
 
-// One unit per WPU waves: a row is LPR = row_bytes / 16 consecutive lanes, 64 / LPR rows per wave and load.
-template <int DT, int WPU>
-__global__ __launch_bounds__(kBThreads) void bounds_update_kernel(Lay a, BoundsArgs A, unsigned lpr)
+// a (layer, block, kv head): where its keys are and how many of them count
+struct BoundsUnit { int layer, blk, cnt; unsigned h; };
+__device__ __forceinline__ BoundsUnit bounds_unit(const Lay &a, const BoundsArgs &A, unsigned unit)
+{
+    BoundsUnit U;
+    const unsigned rest = unit / (unsigned)a.KVH, bi = rest % (unsigned)A.n_blocks;
+    U.h = unit - rest * (unsigned)a.KVH;
+    U.layer = A.layer0 + (int)(rest / (unsigned)A.n_blocks);
+    U.blk = -1;
+    U.cnt = 0;
+    const int32_t *tab = A.tables;
+    int pos, lb;
+    if (A.d_pos) {
+        pos = A.d_pos[bi];
+        lb = pos < 0 ? -1 : (int)dv((unsigned)pos, A.bs_div);
+        tab += (size_t)bi * A.table_stride;
+        if (lb >= A.table_stride) lb = -1;
+    } else {
+        lb = A.first_block + (int)bi;
+        pos = A.pos_start + A.n - 1;
+    }
+    if (lb < 0) return U;
+    U.blk = tab[lb];
+    if (U.blk >= 0 && U.blk < a.NB) U.cnt = min(a.bs, pos - lb * a.bs + 1);
+    return U;
+}
+
+// everything above is issued before anything below: the compiler would trade loads in flight for registers
+__device__ __forceinline__ void bounds_issue_barrier()
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_sched_barrier(0);
+#endif
+}
+
+// lowest and highest of 16 bytes of each of the rows r0, r0 + step, .. of a unit; 8 rows in flight
+template <int DT>
+__device__ __forceinline__ void bounds_rows(const Lay &a, const BoundsArgs &A, const BoundsUnit &U, unsigned sub, int r0, int step,
+                                            float *lo, float *hi)
 {
     constexpr int V = BoundsElems<DT>::V;
-    __shared__ float red[WPU > 1 ? 4 : 1][2][V][64];
-    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const unsigned unit = WPU > 1 ? blockIdx.x : blockIdx.x * 4 + w;
-    bool ok = unit < A.units;
-    const unsigned h = unit % (unsigned)a.KVH, rest = unit / (unsigned)a.KVH;
-    const unsigned nb = (unsigned)A.n_blocks, bi = rest % nb;
-    const int layer = A.layer0 + (int)(rest / nb);
-    int cnt = 0, blk = -1;
-    if (ok) {
-        int pos, lb;
-        const int32_t *tab = A.tables;
-        if (A.d_pos) {
-            pos = A.d_pos[bi];
-            lb = pos < 0 ? -1 : (int)dv((unsigned)pos, A.bs_div);
-            tab += (size_t)bi * A.table_stride;
-            if (lb >= A.table_stride) lb = -1;
-        } else {
-            lb = A.first_block + (int)bi;
-            pos = A.pos_start + A.n - 1;
-        }
-        if (lb >= 0) {
-            blk = tab[lb];
-            cnt = min(a.bs, pos - lb * a.bs + 1);
-        }
-        ok = blk >= 0 && blk < a.NB;
-    }
-    if (!ok) cnt = 0;
-    const unsigned sub = lane % lpr, r0 = lane / lpr, rpw = 64 / lpr;
-    float lo[V], hi[V];
 #pragma unroll
     for (int i = 0; i < V; i++) { lo[i] = INFINITY; hi[i] = -INFINITY; }
-    if (ok) {
-        const uint8_t *base = A.pool + row_off(a, layer, blk, 0, (int)h, 0);
-        const uint8_t *sc = A.pool + (DT == DRK_INT8 ? scale_off(a, layer, blk, 0, (int)h, 0) : 0);
-        const int step = (int)rpw * WPU;
-        for (int r = (int)r0 + (WPU > 1 ? w * (int)rpw : 0); r < cnt; r += 4 * step) {
-            uint4 v[4];
-            float s[4];
+    if (r0 >= U.cnt) return;
+    const uint8_t *base = A.pool + row_off(a, U.layer, U.blk, 0, (int)U.h, 0) + sub * 16;
+    const uint8_t *sc = A.pool + (DT == DRK_INT8 ? scale_off(a, U.layer, U.blk, 0, (int)U.h, 0) : 0);
+    for (int r = r0; r < U.cnt; r += 8 * step) {
+        uint4 v[8];
+        float s[8];
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                const int rr = min(r + u * step, cnt - 1);         // a row read twice changes no bound
-                v[u] = ld_stream128(base + (size_t)rr * a.row_bytes + sub * 16);
-                s[u] = DT == DRK_INT8 ? f16_bits_to_f(*(const uint16_t *)(sc + (size_t)rr * 2)) : 1.0f;
-            }
+        for (int u = 0; u < 8; u++) {
+            const int rr = min(r + u * step, U.cnt - 1);               // a row read twice changes no bound
+            v[u] = ld_stream128(base + (size_t)rr * a.row_bytes);
+            s[u] = DT == DRK_INT8 ? f16_bits_to_f(*(const uint16_t *)(sc + (size_t)rr * 2)) : 1.0f;
+        }
+        bounds_issue_barrier();
 #pragma unroll
-            for (int u = 0; u < 4; u++) {
-                float x[V];
-                bounds_unpack<DT>(v[u], s[u], x);
+        for (int u = 0; u < 8; u++) {
+            float x[V];
+            bounds_unpack<DT>(v[u], s[u], x);
 #pragma unroll
-                for (int i = 0; i < V; i++) { lo[i] = fminf(lo[i], x[i]); hi[i] = fmaxf(hi[i], x[i]); }
-            }
+            for (int i = 0; i < V; i++) { lo[i] = fminf(lo[i], x[i]); hi[i] = fmaxf(hi[i], x[i]); }
         }
     }
-    for (unsigned off = lpr; off < 64; off <<= 1)
-#pragma unroll
-        for (int i = 0; i < V; i++) {
-            lo[i] = fminf(lo[i], __shfl_xor(lo[i], (int)off));
-            hi[i] = fmaxf(hi[i], __shfl_xor(hi[i], (int)off));
-        }
-    if constexpr (WPU > 1) {
-#pragma unroll
-        for (int i = 0; i < V; i++) { red[w][0][i][lane] = lo[i]; red[w][1][i][lane] = hi[i]; }
-        __syncthreads();
-        if (w) return;
-#pragma unroll
-        for (int i = 0; i < V; i++)
-            for (int k = 1; k < 4; k++) {
-                lo[i] = fminf(lo[i], red[k][0][i][lane]);
-                hi[i] = fmaxf(hi[i], red[k][1][i][lane]);
-            }
-    }
+}
+
+__device__ __forceinline__ uint32_t bounds_code(float x, int e, bool high)
+{
+    const float y = fminf(fmaxf(ldexpf(x, -e), -127.0f), 127.0f);
+    return (uint32_t)(int)(high ? ceilf(y) : floorf(y)) & 0xffu;
+}
+
+// Short blocks: a thread owns 16 bytes of every row of its unit, so nothing is exchanged but the largest magnitude;
+// row_bytes / 16 neighbouring lanes hold a unit.
+template <int DT>
+__global__ __launch_bounds__(kBThreads) void bounds_update_kernel(Lay a, BoundsArgs A, unsigned lpr, int lpr_shift)
+{
+    constexpr int V = BoundsElems<DT>::V;
+    const size_t i0 = (size_t)blockIdx.x * kBThreads + threadIdx.x;
+    const size_t unit = i0 >> lpr_shift;
+    const unsigned sub = (unsigned)i0 & (lpr - 1);
+    BoundsUnit U = {0, -1, 0, 0};
+    if (unit < A.units) U = bounds_unit(a, A, (unsigned)unit);
+    float lo[V], hi[V];
+    bounds_rows<DT>(a, A, U, sub, 0, 1, lo, hi);
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        if (lo[i] > hi[i]) lo[i] = hi[i] = 0.0f;                      // nothing but NaN
+        if (lo[i] > hi[i]) lo[i] = hi[i] = 0.0f;                       // nothing but NaN
         amax = fmaxf(amax, fmaxf(fabsf(lo[i]), fabsf(hi[i])));
     }
     for (unsigned off = lpr >> 1; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, (int)off));
-    if (!ok || (unsigned)lane >= lpr) return;
+    if (U.cnt <= 0) return;
     const int e = bounds_exponent(amax);
     uint32_t cl[V / 4], ch[V / 4];
 #pragma unroll
@@ -142,13 +152,11 @@ __global__ __launch_bounds__(kBThreads) void bounds_update_kernel(Lay a, BoundsA
         cl[i] = ch[i] = 0;
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            const float l = floorf(fminf(fmaxf(ldexpf(lo[4 * i + j], -e), -127.0f), 127.0f));
-            const float g = ceilf(fminf(fmaxf(ldexpf(hi[4 * i + j], -e), -127.0f), 127.0f));
-            cl[i] |= ((uint32_t)(int)l & 0xffu) << (8 * j);
-            ch[i] |= ((uint32_t)(int)g & 0xffu) << (8 * j);
+            cl[i] |= bounds_code(lo[4 * i + j], e, false) << (8 * j);
+            ch[i] |= bounds_code(hi[4 * i + j], e, true) << (8 * j);
         }
     }
-    const size_t entry = ((size_t)layer * a.NB + blk) * a.KVH + h;
+    const size_t entry = ((size_t)U.layer * a.NB + U.blk) * a.KVH + U.h;
     uint8_t *dst = A.bounds + entry * 2 * a.D + sub * V;
     if constexpr (V == 8) {
         *(uint2 *)dst = make_uint2(cl[0], cl[1]);
@@ -158,6 +166,52 @@ __global__ __launch_bounds__(kBThreads) void bounds_update_kernel(Lay a, BoundsA
         *(uint4 *)(dst + a.D) = make_uint4(ch[0], ch[1], ch[2], ch[3]);
     }
     if (sub == 0) A.bounds[A.exps + entry] = (uint8_t)(int8_t)e;
+}
+
+// Long blocks: a workgroup per unit, its rows dealt out to 256 / lpr threads per 16-byte column; the partial bounds meet
+// in LDS, where thread d then owns dimension d.
+template <int DT>
+__global__ __launch_bounds__(kBThreads) void bounds_update_long_kernel(Lay a, BoundsArgs A, unsigned lpr, int lpr_shift)
+{
+    constexpr int V = BoundsElems<DT>::V;
+    __shared__ __align__(16) float red[2][kBThreads * V];              // [low, high][row group][dimension]
+    __shared__ float wmax[4];
+    const BoundsUnit U = bounds_unit(a, A, blockIdx.x);
+    if (U.cnt <= 0) return;                                            // the same for the whole workgroup
+    const unsigned sub = threadIdx.x & (lpr - 1), rg = threadIdx.x >> lpr_shift;
+    const int groups = (int)(kBThreads >> lpr_shift);
+    float lo[V], hi[V];
+    bounds_rows<DT>(a, A, U, sub, (int)rg, groups, lo, hi);
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+        *(float4 *)&red[0][rg * a.D + sub * V + i] = make_float4(lo[i], lo[i + 1], lo[i + 2], lo[i + 3]);
+        *(float4 *)&red[1][rg * a.D + sub * V + i] = make_float4(hi[i], hi[i + 1], hi[i + 2], hi[i + 3]);
+    }
+    __syncthreads();
+    float l[2], g[2], amax = 0.0f;                                     // head_dim is at most 512
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int d = (int)threadIdx.x + k * kBThreads;
+        l[k] = INFINITY;
+        g[k] = -INFINITY;
+        if (d >= a.D) continue;
+        for (int r = 0; r < groups; r++) { l[k] = fminf(l[k], red[0][r * a.D + d]); g[k] = fmaxf(g[k], red[1][r * a.D + d]); }
+        if (l[k] > g[k]) l[k] = g[k] = 0.0f;
+        amax = fmaxf(amax, fmaxf(fabsf(l[k]), fabsf(g[k])));
+    }
+    for (int off = 32; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off));
+    if ((threadIdx.x & 63) == 0) wmax[threadIdx.x >> 6] = amax;
+    __syncthreads();
+    const int e = bounds_exponent(fmaxf(fmaxf(wmax[0], wmax[1]), fmaxf(wmax[2], wmax[3])));
+    const size_t entry = ((size_t)U.layer * a.NB + U.blk) * a.KVH + U.h;
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+        const int d = (int)threadIdx.x + k * kBThreads;
+        if (d >= a.D) continue;
+        A.bounds[entry * 2 * a.D + d] = (uint8_t)bounds_code(l[k], e, false);
+        A.bounds[entry * 2 * a.D + a.D + d] = (uint8_t)bounds_code(g[k], e, true);
+    }
+    if (threadIdx.x == 0) A.bounds[A.exps + entry] = (uint8_t)(int8_t)e;
 }
 
 // 16 codes per thread -> 16 bf16 values (7 bits and a power of two: exact)
@@ -234,16 +288,17 @@ int drk_kv_bounds_update(const drk_kv_layout *g, const void *pool, const int32_t
     A.first_block = d_pos ? 0 : pos_start / a.bs;
     A.n_blocks = d_pos ? n : (pos_start + n - 1) / a.bs - A.first_block + 1;
     const size_t units = (size_t)A.n_blocks * a.KVH * layer_count;
-    if (units > 0x7fffffffu) return fail(DRK_ERR_INVALID, "kv_bounds_update: too many blocks");
+    if (units * (a.row_bytes / 16) > ((size_t)0x7fffffff << 8) || units > 0x7fffffffu) return fail(DRK_ERR_INVALID, "kv_bounds_update: too many blocks");
     A.units = (unsigned)units;
     const unsigned lpr = a.row_bytes / 16;
-    const bool wide = (size_t)a.head_stride > 8192;
-    const dim3 grid(wide ? (unsigned)units : (unsigned)((units + 3) / 4));
+    const int lpr_shift = ilog2_exact(lpr);
+    const bool wide = a.bs > kBLongBlock;
+    const dim3 grid(wide ? (unsigned)units : (unsigned)((units * lpr + kBThreads - 1) / kBThreads));
     hipStream_t st = (hipStream_t)stream;
-#define DRK_BOUNDS_LAUNCH(DT)                                                                                                     \
-    do {                                                                                                                          \
-        if (wide) hipLaunchKernelGGL((bounds_update_kernel<DT, 4>), grid, dim3(kBThreads), 0, st, a, A, lpr);                     \
-        else hipLaunchKernelGGL((bounds_update_kernel<DT, 1>), grid, dim3(kBThreads), 0, st, a, A, lpr);                          \
+#define DRK_BOUNDS_LAUNCH(DT)                                                                                             \
+    do {                                                                                                                  \
+        if (wide) hipLaunchKernelGGL(bounds_update_long_kernel<DT>, grid, dim3(kBThreads), 0, st, a, A, lpr, lpr_shift);  \
+        else hipLaunchKernelGGL(bounds_update_kernel<DT>, grid, dim3(kBThreads), 0, st, a, A, lpr, lpr_shift);            \
     } while (0)
     switch (a.dtype) {
     case DRK_F16: DRK_BOUNDS_LAUNCH(DRK_F16); break;

@@ -15,6 +15,7 @@
 namespace drk {
 
 constexpr int kRThreads = 256;
+constexpr size_t kRopeShare = 1 << 18;    // threads from which one takes four head rows
 
 // f'_i, see drk_rope in drk_kv.h
 __device__ __forceinline__ double rope_turns(const drk_rope &r, int i)
@@ -62,7 +63,7 @@ struct RopeArgs {
     const double *freqs;
     const int32_t *d_pos;
     int first_head[DRK_ROPE_MAX_TENSORS];   // head rows before tensor i in a token's list of them
-    int n_tensors, pos_start, T, rows, units, hp, interleaved, dtype;
+    int n_tensors, pos_start, T, rows, row_groups, units, hp, interleaved;
     float cm, sm;                           // factors of cos and sin: the magnitude, and its sign turned for the inverse
 };
 
@@ -70,61 +71,82 @@ __device__ __forceinline__ uint4 rope_pack8(const float *y, int dtype)
 {
     uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        w[i] = (uint32_t)f_to_elem16(y[2 * i], dtype) | ((uint32_t)f_to_elem16(y[2 * i + 1], dtype) << 16);
+    for (int i = 0; i < 4; i++) {
+        if (dtype == DRK_BF16)
+            w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (__bf16)y[2 * i]) | ((uint32_t)__builtin_bit_cast(uint16_t, (__bf16)y[2 * i + 1]) << 16);
+        else
+            w[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)y[2 * i]) | ((uint32_t)__builtin_bit_cast(uint16_t, (_Float16)y[2 * i + 1]) << 16);
+    }
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// One thread: 8 pairs (or 16 elements that pass unchanged) of one head row.
+// One thread: 8 pairs (or 16 elements that pass unchanged) of HPT head rows of one token, whose angles are the
+// same: the sines, about half of the arithmetic of a row by itself, are formed once.  The heads of a token are
+// taken HPT-strided groups apart, so that neighbouring lanes stay on neighbouring bytes.
+template <int HPT, int DTYPE>
 __global__ __launch_bounds__(kRThreads) void rope_apply_kernel(RopeArgs A)
 {
     const size_t it = (size_t)blockIdx.x * kRThreads + threadIdx.x;
-    if (it >= (size_t)A.T * A.rows * A.units) return;
+    if (it >= (size_t)A.T * A.row_groups * A.units) return;
     const size_t row = it / A.units;
     const int u = (int)(it - row * A.units);
-    const int t = (int)(row / A.rows);
-    int h = (int)(row - (size_t)t * A.rows), n = 0;
-    while (n + 1 < A.n_tensors && h >= A.first_head[n + 1]) n++;
-    h -= A.first_head[n];
-    const drk_rope_rows &R = A.tensors[n];
-    const uint16_t *x = (const uint16_t *)R.x + (size_t)t * R.x_token_stride + (size_t)h * R.x_head_stride;
-    uint16_t *o = (uint16_t *)R.out + (size_t)t * R.out_token_stride + (size_t)h * R.out_head_stride;
-    if (u >= A.hp) {                                   // behind the rotary part
-        const uint4 v0 = *(const uint4 *)(x + u * 16), v1 = *(const uint4 *)(x + u * 16 + 8);
-        *(uint4 *)(o + u * 16) = v0;
-        *(uint4 *)(o + u * 16 + 8) = v1;
-        return;
+    const int t = (int)(row / A.row_groups), h0 = (int)(row - (size_t)t * A.row_groups);
+    const bool rotated = u < A.hp;
+    // half-half: pair (i, i + r/2), so 8 pairs are chunks u and u + hp of 8; interleaved, or behind the rotary part: 16
+    // consecutive elements
+    const int e0 = A.interleaved || !rotated ? u * 16 : u * 8, e1 = A.interleaved || !rotated ? e0 + 8 : e0 + A.hp * 8;
+    uint4 va[HPT], vb[HPT];
+    uint16_t *o[HPT];
+#pragma unroll
+    for (int i = 0; i < HPT; i++) {
+        int h = h0 + i * A.row_groups, n = 0;
+        if (h >= A.rows) { o[i] = nullptr; continue; }
+        while (n + 1 < A.n_tensors && h >= A.first_head[n + 1]) n++;
+        h -= A.first_head[n];
+        const drk_rope_rows &R = A.tensors[n];
+        const uint16_t *x = (const uint16_t *)R.x + (size_t)t * R.x_token_stride + (size_t)h * R.x_head_stride;
+        o[i] = (uint16_t *)R.out + (size_t)t * R.out_token_stride + (size_t)h * R.out_head_stride;
+        va[i] = ld_stream128(x + e0);
+        vb[i] = ld_stream128(x + e1);
     }
-    // half-half: pair (i, i + r/2), so 8 pairs are chunks u and u + hp of 8; interleaved: 16 consecutive elements
-    const int e0 = A.interleaved ? u * 16 : u * 8, e1 = A.interleaved ? e0 + 8 : e0 + A.hp * 8;
-    float a[8], b[8], y0[8], y1[8];
-    unpack8(*(const uint4 *)(x + e0), A.dtype, a);
-    unpack8(*(const uint4 *)(x + e1), A.dtype, b);
-    const double p = A.d_pos ? A.d_pos[t] : (double)A.pos_start + t;
     float c[8], s[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        rope_cos_sin(p, A.freqs[u * 8 + i], c[i], s[i]);
-        c[i] *= A.cm;
-        s[i] *= A.sm;
-    }
-    if (A.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            y0[2 * i] = a[2 * i] * c[i] - a[2 * i + 1] * s[i];
-            y0[2 * i + 1] = a[2 * i + 1] * c[i] + a[2 * i] * s[i];
-            y1[2 * i] = b[2 * i] * c[i + 4] - b[2 * i + 1] * s[i + 4];
-            y1[2 * i + 1] = b[2 * i + 1] * c[i + 4] + b[2 * i] * s[i + 4];
-        }
-    } else {
+    if (rotated) {
+        const double p = A.d_pos ? A.d_pos[t] : (double)A.pos_start + t;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            y0[i] = a[i] * c[i] - b[i] * s[i];
-            y1[i] = b[i] * c[i] + a[i] * s[i];
+            rope_cos_sin(p, A.freqs[u * 8 + i], c[i], s[i]);
+            c[i] *= A.cm;
+            s[i] *= A.sm;
         }
     }
-    *(uint4 *)(o + e0) = rope_pack8(y0, A.dtype);
-    *(uint4 *)(o + e1) = rope_pack8(y1, A.dtype);
+#pragma unroll
+    for (int k = 0; k < HPT; k++) {
+        if (!o[k]) continue;
+        if (rotated) {
+            float a[8], b[8], y0[8], y1[8];
+            unpack8(va[k], DTYPE, a);
+            unpack8(vb[k], DTYPE, b);
+            if (A.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    y0[2 * i] = a[2 * i] * c[i] - a[2 * i + 1] * s[i];
+                    y0[2 * i + 1] = a[2 * i + 1] * c[i] + a[2 * i] * s[i];
+                    y1[2 * i] = b[2 * i] * c[i + 4] - b[2 * i + 1] * s[i + 4];
+                    y1[2 * i + 1] = b[2 * i + 1] * c[i + 4] + b[2 * i] * s[i + 4];
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    y0[i] = a[i] * c[i] - b[i] * s[i];
+                    y1[i] = b[i] * c[i] + a[i] * s[i];
+                }
+            }
+            va[k] = rope_pack8(y0, DTYPE);
+            vb[k] = rope_pack8(y1, DTYPE);
+        }
+        st_stream128(o[k] + e0, va[k]);
+        st_stream128(o[k] + e1, vb[k]);
+    }
 }
 
 static int check_rope(const drk_rope *r, const char *who)
@@ -204,13 +226,23 @@ int drk_rope_apply(const drk_rope *r, const double *d_freqs, const drk_rope_rows
     A.freqs = d_freqs; A.d_pos = d_pos; A.n_tensors = n_tensors; A.pos_start = pos_start; A.T = T;
     A.hp = r->rotary_dim / 16;
     A.units = in_place ? A.hp : head_dim / 16;              // in place, what passes unchanged is there already
-    A.interleaved = r->interleaved; A.dtype = dtype;
+    A.interleaved = r->interleaved;
     A.cm = r->magnitude; A.sm = inverse ? -r->magnitude : r->magnitude;
-    const size_t items = (size_t)T * A.rows * A.units;
-    if (items == 0) return DRK_OK;
-    const size_t blocks = (items + kRThreads - 1) / kRThreads;
+    const size_t all = (size_t)T * A.rows * A.units;
+    if (all == 0) return DRK_OK;
+    const int hpt = all >= kRopeShare ? 4 : 1;
+    A.row_groups = (A.rows + hpt - 1) / hpt;
+    const size_t blocks = ((size_t)T * A.row_groups * A.units + kRThreads - 1) / kRThreads;
     if (blocks > 0x7fffffffu) return fail(DRK_ERR_INVALID, "rope_apply: too many rows");
-    hipLaunchKernelGGL(rope_apply_kernel, dim3((unsigned)blocks), dim3(kRThreads), 0, (hipStream_t)stream, A);
+    const dim3 grid((unsigned)blocks);
+    hipStream_t st = (hipStream_t)stream;
+    if (dtype == DRK_BF16) {
+        if (hpt == 4) hipLaunchKernelGGL((rope_apply_kernel<4, DRK_BF16>), grid, dim3(kRThreads), 0, st, A);
+        else hipLaunchKernelGGL((rope_apply_kernel<1, DRK_BF16>), grid, dim3(kRThreads), 0, st, A);
+    } else {
+        if (hpt == 4) hipLaunchKernelGGL((rope_apply_kernel<4, DRK_F16>), grid, dim3(kRThreads), 0, st, A);
+        else hipLaunchKernelGGL((rope_apply_kernel<1, DRK_F16>), grid, dim3(kRThreads), 0, st, A);
+    }
     DRK_LAUNCH_CHECK("rope_apply_kernel");
     return DRK_OK;
 }

@@ -7,14 +7,17 @@
 // power of two -- exact in fp32, the same for every order of summation, and the selection cannot
 // depend on how the work was cut.
 //
-// score_kernel: a wave takes 16 blocks as the rows of v_mfma_i32_16x16x64_i8 -- a block's codes lie
-// as the operand wants them, 16 bytes per lane -- and 16 columns: the query heads of a kv head (padded to
-// a power of two by repeating the last) of one row, or of several rows when all rows share one table.
-// It leaves an ordered 32-bit key per block: 0 = not a candidate, 2^32 - 1 = always kept, otherwise
-// the score's bits in an order-preserving form.
-// topk_kernel: one workgroup per (row, kv head) finds the n_keep-th key by histograms of 2048 bins over
-// the range the keys really span (a handful of keys remain after the first) and writes the chosen
-// indices in ascending order by prefix sums of ballots: no atomics decide an order.
+// The score kernels form v_mfma_i32_16x16x64_i8 products of 16 query heads (rows) with 16 blocks (columns): a
+// block's codes lie as the operand wants them, 16 bytes per lane, and the result has a block per lane and
+// four heads in its registers, so the largest score over a kv head's heads is mostly formed in a lane.  They
+// leave an ordered 32-bit key per block: 0 = not a candidate, 2^32 - 1 = always kept, otherwise the score's
+// bits in an order-preserving form.
+//   score_kernel: a wave scores its own blocks for one set of 16 heads -- branches, whose blocks nobody else
+//   reads.  Bound by the bytes of the bounds.
+//   score_tile_kernel: rows of one table; 8 waves x 2 sets of heads meet the same blocks, which pass through LDS.
+// topk_kernel: one workgroup per (row, kv head) finds the n_keep-th key: a histogram over the range the keys
+// really span leaves a handful in one bin, which every wave then settles by itself with ballots; the chosen
+// indices are written in ascending order by prefix sums of ballots.  No atomic decides an order.
 #include "drk_common.hpp"
 #include "drk_codec.hpp"
 #include "drk_bounds.hpp"
@@ -22,6 +25,8 @@
 namespace drk {
 
 constexpr uint32_t kKeyForced = 0xffffffffu;
+constexpr int kSelFused = 1024;         // blocks of a context up to which one workgroup scores and selects
+constexpr size_t kSelWaves = 8192, kSelTileWgs = 512;     // waves / workgroups the scores are spread over
 typedef int sel_i32x4 __attribute__((ext_vector_type(4)));
 
 struct SelArgs {
@@ -31,7 +36,7 @@ struct SelArgs {
     uint32_t *keys;                     // [T][KVH][key_stride]
     int32_t *out;
     int table_stride, pos_start, T, max_seq_len, keep, sink, recent, io_dtype;
-    int P, R;                           // columns per row (a power of two >= heads per kv head), rows per 16 columns
+    int P, R;                           // operand rows per query row (a power of two >= heads per kv head), query rows per 16
     int groups_per_wave;
     unsigned key_stride;
     Div bs_div;
@@ -50,266 +55,521 @@ __device__ __forceinline__ uint32_t sel_key(float s)
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// c = rint(x * 2^-e) of 4 values as bytes, split into the negative and the positive part
-__device__ __forceinline__ void sel_codes4(const float *x, float inv, uint32_t &neg, uint32_t &pos)
+// ---- query heads as an operand ----------------------------------------------------------------------
+// Codes c = rint(q 2^-eq) of one head row; lane (c, g) holds dims 64 k + 16 g .. + 15: the negative parts meet the
+// lows (first D / 64 steps), the positive parts the highs.
+template <int D>
+__device__ __forceinline__ int sel_query(const uint8_t *row, int g, int io_dtype, sel_i32x4 *qa)
 {
-    neg = pos = 0;
+    constexpr int HK = D / 64;
+    uint4 raw[HK][2];
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int c = (int)rintf(fminf(fmaxf(x[i] * inv, -127.0f), 127.0f));
-        neg |= ((uint32_t)min(c, 0) & 0xffu) << (8 * i);
-        pos |= ((uint32_t)max(c, 0) & 0xffu) << (8 * i);
+    for (int k = 0; k < HK; k++) {
+        raw[k][0] = *(const uint4 *)(row + k * 128 + g * 32);
+        raw[k][1] = *(const uint4 *)(row + k * 128 + g * 32 + 16);
     }
+    float amax = 0.0f;
+#pragma unroll
+    for (int k = 0; k < HK; k++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            float x[8];
+            unpack8(raw[k][j], io_dtype, x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));        // NaN is passed over
+        }
+    amax = fmaxf(amax, __shfl_xor(amax, 16));
+    amax = fmaxf(amax, __shfl_xor(amax, 32));
+    const int e = bounds_exponent(amax);
+    const float inv = ldexpf(1.0f, -e);
+#pragma unroll
+    for (int k = 0; k < HK; k++) {
+        uint32_t n[4], p[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float x[8];
+            uint32_t u[4];
+            unpack8(raw[k][j >> 1], io_dtype, x);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float y = x[4 * (j & 1) + i] * inv;
+                y = fminf(fmaxf(y == y ? y : 0.0f, -127.0f), 127.0f);
+                u[i] = __float_as_uint(__fadd_rn(y, 12582912.0f));              // 1.5 * 2^23: rounds to even, the code is the low byte
+            }
+            const uint32_t c = s_perm(s_perm(u[3], u[2], 0x04000c0cu), s_perm(u[1], u[0], 0x0c0c0400u), 0x07060100u);
+            const uint32_t s = (c >> 7) & 0x01010101u, mask = (s << 8) - s;     // 0xff in the negative codes' bytes
+            n[j] = c & mask;
+            p[j] = c & ~mask;
+        }
+        qa[k] = sel_i32x4{(int)n[0], (int)n[1], (int)n[2], (int)n[3]};
+        qa[HK + k] = sel_i32x4{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
+    }
+    return e;
 }
 
-template <int D, int SETS>
+__device__ __forceinline__ float sel_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Heads 4g + j of one product against block c: the largest score over the P heads of a row (P = 4, 8 or 16), valid in every
+// lane of the row.  qm = 2^eq of the heads, bm = 2^e of the block.
+__device__ __forceinline__ float sel_row_max(const sel_i32x4 &acc, const float *qm, int P, float bm)
+{
+    float x = fmaxf(fmaxf((float)acc[0] * qm[0], (float)acc[1] * qm[1]), fmaxf((float)acc[2] * qm[2], (float)acc[3] * qm[3]));
+#if defined(__HIP_DEVICE_COMPILE__)
+    // a row's other heads are 16 (and 32) lanes away: the two results of a swap with itself are the two sides
+    if (P >= 8) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    }
+    if (P >= 16) {
+        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    }
+#endif
+    return x * bm;
+}
+
+constexpr int kNoBlock = 1000;          // in place of the exponent of a block without a page
+
+__device__ __forceinline__ uint32_t sel_key_of(const SelArgs &A, float x, int b, int nb, int e)
+{
+    if (b >= nb || e == kNoBlock) return 0u;
+    return b < A.sink || b >= nb - A.recent ? kKeyForced : sel_key(x);
+}
+
+// One set of 16 heads per wave: a branch's row (R = 1), or R = 16 / P rows of one table.
+template <int D>
 __global__ __launch_bounds__(256) void score_kernel(Lay a, SelArgs A)
 {
-    constexpr int HK = D / 64, KS = 2 * HK;                  // 64-byte steps of one half / of a row of codes
+    constexpr int KS = D / 32;
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
-    const int h = blockIdx.y, GQ = a.QH / a.KVH;
-    const int row0 = blockIdx.z * (A.R * SETS);
-    const int first = ((int)blockIdx.x * 4 + w) * A.groups_per_wave;      // first 16-block group of this wave
-
-    // the columns: codes of one query head each, the negative parts against the lows, the positive against the highs
-    sel_i32x4 qb[SETS][KS];
-    int eq[SETS], nbr[SETS], trow[SETS];
-    int nbmax = 0;
-#pragma unroll
-    for (int s = 0; s < SETS; s++) {
-        const int t = row0 + s * A.R + (A.R > 1 ? c / A.P : 0);
-        trow[s] = t;
-        nbr[s] = t < A.T ? sel_blocks_of_row(A, t) : 0;
-        nbmax = max(nbmax, nbr[s]);
-    }
-#pragma unroll
-    for (int off = 1; off < 16; off <<= 1) nbmax = max(nbmax, __shfl_xor(nbmax, off));
-    if (first * 16 >= nbmax) return;
-#pragma unroll
-    for (int s = 0; s < SETS; s++) {
-        const int t = min(trow[s], A.T - 1), head = h * GQ + min(c % A.P, GQ - 1);
-        const uint8_t *qp = A.q + ((size_t)t * a.QH + head) * D * 2 + g * 32;
-        float x[HK][16], amax = 0.0f;
-#pragma unroll
-        for (int k = 0; k < HK; k++) {
-            unpack8(*(const uint4 *)(qp + k * 128), A.io_dtype, &x[k][0]);
-            unpack8(*(const uint4 *)(qp + k * 128 + 16), A.io_dtype, &x[k][8]);
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                x[k][i] = x[k][i] == x[k][i] ? x[k][i] : 0.0f;
-                amax = fmaxf(amax, fabsf(x[k][i]));
-            }
-        }
-        amax = fmaxf(amax, __shfl_xor(amax, 16));
-        amax = fmaxf(amax, __shfl_xor(amax, 32));
-        eq[s] = bounds_exponent(amax);
-        const float inv = ldexpf(1.0f, -eq[s]);
-#pragma unroll
-        for (int k = 0; k < HK; k++) {
-            uint32_t n[4], p[4];
-#pragma unroll
-            for (int i = 0; i < 4; i++) sel_codes4(&x[k][4 * i], inv, n[i], p[i]);
-            qb[s][k] = sel_i32x4{(int)n[0], (int)n[1], (int)n[2], (int)n[3]};
-            qb[s][HK + k] = sel_i32x4{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
-        }
-    }
+    const int h = blockIdx.x, GQ = a.QH / a.KVH;           // kv heads vary fastest: a block's codes of all heads lie together
+    const int row0 = blockIdx.z * A.R;
+    const int first = ((int)blockIdx.y * 4 + w) * A.groups_per_wave;
     const int32_t *tab = A.tables + (size_t)row0 * A.table_stride;
+    // the row of this lane's results (heads 4g .. 4g + 3), and the wave's longest
+    const int row = A.R > 1 ? row0 + 4 * g / A.P : row0;
+    const int nbr = row < A.T ? sel_blocks_of_row(A, row) : 0;
+    const int nbmax = max(max(__shfl(nbr, 0), __shfl(nbr, 16)), max(__shfl(nbr, 32), __shfl(nbr, 48)));
+    if (first * 16 >= nbmax) return;
+    int ahead = first * 16 + lane < nbmax ? tab[first * 16 + lane] : -1;       // the table entries of four groups
 
-    for (int gi = first; gi < first + A.groups_per_wave && gi * 16 < nbmax; gi++) {
-        const int lb = gi * 16 + c;                          // this lane's block as an operand row
-        int blk = lb < nbmax ? tab[lb] : -1;
+    const int qrow = min(A.R > 1 ? row0 + c / A.P : row0, A.T - 1);
+    sel_i32x4 qa[KS];
+    const int eq = sel_query<D>(A.q + ((size_t)qrow * a.QH + h * GQ + min(c & (A.P - 1), GQ - 1)) * D * 2, g, A.io_dtype, qa);
+    float qm[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) qm[j] = sel_pow2(__shfl(eq, 4 * g + j));
+
+    uint4 bv[KS];
+    int eb = 0;
+    auto fetch = [&](int i) {                                                   // group first + i; ahead holds its entries
+        const int blk = __shfl(ahead, (i & 3) * 16 + c);
         const bool hole = blk < 0 || blk >= a.NB;
-        if (hole) blk = 0;                                   // always mapped; its score is not used
-        const size_t entry = (size_t)blk * a.KVH + h;
+        const size_t entry = (size_t)(hole ? 0 : blk) * a.KVH + h;              // block 0 is always mapped; its score is not used
         const uint8_t *cp = A.bounds + entry * (2 * D) + g * 16;
-        uint4 av[KS];
 #pragma unroll
-        for (int k = 0; k < KS; k++) av[k] = *(const uint4 *)(cp + k * 64);
-        const int eb = hole ? 1000 : (int)(int8_t)A.exps[entry];
-        int ebj[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) ebj[j] = __shfl(eb, 4 * g + j);
-#pragma unroll
-        for (int s = 0; s < SETS; s++) {
-            sel_i32x4 acc = {0, 0, 0, 0};
+        for (int k = 0; k < KS; k++) bv[k] = *(const uint4 *)(cp + k * 64);
+        eb = hole ? kNoBlock : (int)(int8_t)A.exps[entry];
+    };
+    fetch(0);
+    const int n = min(A.groups_per_wave, (nbmax + 15) / 16 - first);
+    for (int i = 0; i < n; i++) {
+        sel_i32x4 acc = {0, 0, 0, 0};
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
-            for (int k = 0; k < KS; k++)
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(sel_i32x4, av[k]), qb[s][k], acc, 0, 0, 0);
+        for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[k], __builtin_bit_cast(sel_i32x4, bv[k]), acc, 0, 0, 0);
 #endif
-            uint32_t key[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float x = ldexpf((float)acc[j], ebj[j] == 1000 ? 0 : ebj[j] + eq[s]);
-                for (int off = 1; off < A.P; off <<= 1) x = fmaxf(x, __shfl_xor(x, off));
-                const int b = gi * 16 + 4 * g + j;
-                key[j] = b >= nbr[s] || ebj[j] == 1000 ? 0u : (b < A.sink || b >= nbr[s] - A.recent ? kKeyForced : sel_key(x));
+        const int e = eb;
+        if (i + 1 < n) {
+            if (((i + 1) & 3) == 0) {
+                const int at = (first + i + 1) * 16 + lane;
+                ahead = at < nbmax ? tab[at] : -1;
             }
-            if (c % A.P == 0 && (A.R > 1 || c == 0) && trow[s] < A.T && (unsigned)(gi * 16 + 4 * g) < A.key_stride)
-                *(uint4 *)(A.keys + ((size_t)trow[s] * a.KVH + h) * A.key_stride + gi * 16 + 4 * g) = make_uint4(key[0], key[1], key[2], key[3]);
+            fetch(i + 1);
         }
+        const float x = sel_row_max(acc, qm, A.P, e == kNoBlock ? 0.0f : sel_pow2(e));
+        const int b = (first + i) * 16 + c;
+        if ((A.R > 1 ? ((4 * g) & (A.P - 1)) == 0 : g == 0) && row < A.T && (unsigned)b < A.key_stride)
+            A.keys[((size_t)row * a.KVH + h) * A.key_stride + b] = sel_key_of(A, x, b, nbr, e);
     }
 }
 
-constexpr int kSelBins = 2048;
-
-template <int THREADS>
-__global__ __launch_bounds__(THREADS) void topk_kernel(SelArgs A, int KVH)
+// Rows of one table.  A workgroup's 8 waves hold SETS sets of 16 heads each (8 SETS R rows together) and walk the same
+// blocks, 32 at a time, whose codes the workgroup stages in LDS, two buffers by turns, requested two steps ahead: every
+// byte of the bounds is read once per 8 SETS R rows.
+template <int D, int SETS>
+__global__ __launch_bounds__(512) void score_tile_kernel(Lay a, SelArgs A)
 {
-    constexpr int W = THREADS / 64, NR = 8, BPT = kSelBins / THREADS, SLAB = NR * THREADS;
-    __shared__ uint32_t hist[kSelBins];
-    __shared__ uint32_t red[4][W];
-    __shared__ uint32_t cgt[NR * W], ceq[NR * W];
-    __shared__ uint32_t found[3];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int t = blockIdx.x / KVH;
-    const int nb = sel_blocks_of_row(A, t);
-    const uint32_t *keys = A.keys + (size_t)blockIdx.x * A.key_stride;
-    int32_t *out = A.out + (size_t)blockIdx.x * A.keep;
-    const int slabs = (nb + SLAB - 1) / SLAB;
-    uint32_t kr[NR];
-    auto load = [&](int sl) {
+    constexpr int KS = D / 32, CH = 2 * D / 16;              // 16-byte chunks of a block's codes
+    constexpr int PITCH = 2 * D + 16, G = 2, PER = (16 * G * CH + 511) / 512;
+    static_assert(512 % CH == 0, "a thread's chunks are the same one of several blocks");
+    __shared__ __align__(16) uint8_t b_lds[2][16 * G * PITCH];
+    __shared__ int e_lds[2][16 * G];
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int h = blockIdx.x, GQ = a.QH / a.KVH;
+    const int row0 = (int)blockIdx.z * (8 * SETS * A.R), wrow0 = row0 + w * SETS * A.R;
+    const int first = (int)blockIdx.y * A.groups_per_wave;   // 16-block groups; a workgroup takes an even number
+    const int last_row = min(row0 + 8 * SETS * A.R, A.T) - 1;
+    // lengths may be any where they are given: the workgroup walks to its longest row
+    int nbmax = 0;
+    for (int r = row0 + lane; r <= last_row; r += 64) nbmax = max(nbmax, sel_blocks_of_row(A, r));
 #pragma unroll
-        for (int i = 0; i < NR; i++) {
-            const int idx = sl * SLAB + i * THREADS + tid;
-            kr[i] = idx < nb ? keys[idx] : 0u;
+    for (int off = 1; off < 64; off <<= 1) nbmax = max(nbmax, __shfl_xor(nbmax, off));
+    if (first * 16 >= nbmax) return;
+    const int n = (min(A.groups_per_wave, (nbmax + 15) / 16 - first) + G - 1) / G;         // steps
+
+    // thread (r0, ch) brings chunk ch of blocks r0, r0 + 512 / CH, .. of a step; ahead: their table entries
+    const int r0 = (int)threadIdx.x / CH, ch = (int)threadIdx.x - r0 * CH;
+    uint4 st[2][PER];
+    int es[2][PER], ahead[PER];
+    auto page = [&](int i) {
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const int r = r0 + u * (512 / CH), lb = (first + i * G) * 16 + r;
+            ahead[u] = r < 16 * G && lb < nbmax ? A.tables[lb] : -1;
         }
     };
+    auto fetch = [&](int s) {
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const bool hole = ahead[u] < 0 || ahead[u] >= a.NB;
+            const size_t entry = (size_t)(hole ? 0 : ahead[u]) * a.KVH + h;     // block 0 is always mapped
+            if (r0 + u * (512 / CH) < 16 * G) st[s][u] = *(const uint4 *)(A.bounds + entry * (2 * D) + ch * 16);
+            es[s][u] = hole ? kNoBlock : (ch == 0 ? (int)(int8_t)A.exps[entry] : 0);
+        }
+    };
+    auto stage = [&](int buf) {                               // the older of the two sets in flight
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const int r = r0 + u * (512 / CH);
+            if (r < 16 * G) *(uint4 *)(b_lds[buf] + r * PITCH + ch * 16) = st[0][u];
+            if (r < 16 * G && ch == 0) e_lds[buf][r] = es[0][u];
+            st[0][u] = st[1][u];
+            es[0][u] = es[1][u];
+        }
+    };
+    page(0);
+    fetch(0);
+    page(1);
+    sel_i32x4 qa[SETS][KS];
+    float qm[SETS][4];
+    int nbr[SETS];
+    uint32_t *kp[SETS];
+#pragma unroll
+    for (int s = 0; s < SETS; s++) {
+        const int qrow = min(wrow0 + s * A.R + c / A.P, A.T - 1);
+        const int eq = sel_query<D>(A.q + ((size_t)qrow * a.QH + h * GQ + min(c & (A.P - 1), GQ - 1)) * D * 2, g, A.io_dtype, qa[s]);
+#pragma unroll
+        for (int j = 0; j < 4; j++) qm[s][j] = sel_pow2(__shfl(eq, 4 * g + j));
+        const int row = wrow0 + s * A.R + 4 * g / A.P;
+        nbr[s] = row < A.T ? sel_blocks_of_row(A, row) : 0;
+        kp[s] = ((4 * g) & (A.P - 1)) == 0 && row < A.T ? A.keys + ((size_t)row * a.KVH + h) * A.key_stride : nullptr;
+    }
+    fetch(1);
+    page(2);
+    stage(0);
+    __syncthreads();
+    for (int i = 0; i < n; i++) {
+        fetch(1);
+        page(i + 3);
+        const uint8_t *buf = b_lds[i & 1];
+#pragma unroll
+        for (int x = 0; x < G; x++) {
+            uint4 bv[KS];
+#pragma unroll
+            for (int k = 0; k < KS; k++) bv[k] = *(const uint4 *)(buf + (x * 16 + c) * PITCH + k * 64 + g * 16);
+            const int e = e_lds[i & 1][x * 16 + c], b = (first + i * G + x) * 16 + c;
+            const float bm = e == kNoBlock ? 0.0f : sel_pow2(e);
+#pragma unroll
+            for (int s = 0; s < SETS; s++) {
+                sel_i32x4 acc = {0, 0, 0, 0};
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[s][k], __builtin_bit_cast(sel_i32x4, bv[k]), acc, 0, 0, 0);
+#endif
+                const float y = sel_row_max(acc, qm[s], A.P, bm);
+                if (kp[s] && (unsigned)b < A.key_stride) kp[s][b] = sel_key_of(A, y, b, nbr[s], e);
+            }
+        }
+        stage((i + 1) & 1);
+        __syncthreads();
+    }
+}
+
+// ---- the n_keep best keys ------------------------------------------------------------------------------
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t sel_dpp(uint32_t v)                     // 0 where the source lane does not exist
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, true);
+#else
+    return v;
+#endif
+}
+// inclusive prefix sum over the wave: row shifts by 1, 2, 4, 8, then lane 15 of a row into the next, lane 31 into the rest
+__device__ __forceinline__ uint32_t sel_scan(uint32_t v)
+{
+    v += sel_dpp<0x111, 0xf>(v);
+    v += sel_dpp<0x112, 0xf>(v);
+    v += sel_dpp<0x114, 0xf>(v);
+    v += sel_dpp<0x118, 0xf>(v);
+    v += sel_dpp<0x142, 0xa>(v);
+    v += sel_dpp<0x143, 0xc>(v);
+    return v;
+}
+__device__ __forceinline__ uint32_t sel_lane(uint32_t v, int l)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, l);
+#else
+    (void)l;
+    return v;
+#endif
+}
+__device__ __forceinline__ uint32_t sel_wave_max(uint32_t v)                // the largest, in every lane
+{
+    v = max(v, sel_dpp<0xB1, 0xf>(v));
+    v = max(v, sel_dpp<0x4E, 0xf>(v));
+    v = max(v, sel_dpp<0x141, 0xf>(v));
+    v = max(v, sel_dpp<0x140, 0xf>(v));
+    return max(max(sel_lane(v, 0), sel_lane(v, 16)), max(sel_lane(v, 32), sel_lane(v, 48)));
+}
+
+constexpr uint32_t kSelList = 64;       // keys of the deciding bin that a wave settles by itself
+
+template <int THREADS> struct TopkLds {
+    static constexpr int W = THREADS / 64, BIN_BITS = THREADS >= 1024 ? 11 : 10, BINS = 1 << BIN_BITS;
+    uint32_t hist[BINS], red[4][W], above_w[W], chosen_w[2][W], found[3], list[kSelList], list_n;
+};
+
+// The workgroup's part of one (row, kv head).  Keys come in slabs of NR * THREADS: fetch(slab, kr) leaves NR keys per thread,
+// key i of lane l of wave w being block slab * SLAB + (w * NR + i) * 64 + l (0 from the row's end on) -- a wave's keys are
+// neighbours, so that only one count per wave is exchanged when the chosen ones are written.  The first slab's
+// keys are in kr already; MULTI: there may be more.  (The code runs once per workgroup, so its length is time: about
+// 10 KB of it, with the refetching of slabs in it and the waves' figures added up one by one, cost 6.2 us at 2048 keys.)
+template <int THREADS, int NR, bool MULTI, typename F>
+__device__ __forceinline__ void topk_run(TopkLds<THREADS> &S, uint32_t (&kr)[NR], int nb, int keep, int32_t *out, F fetch)
+{
+    using L = TopkLds<THREADS>;
+    constexpr int W = L::W, BIN_BITS = L::BIN_BITS, BINS = L::BINS, BPT = BINS / THREADS, SLAB = NR * THREADS;
+    static_assert(BPT * THREADS == BINS, "every thread owns whole bins");
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int slabs = MULTI ? (nb + SLAB - 1) / SLAB : 1;
+    auto scored = [](uint32_t k) { return k - 1u < kKeyForced - 1u; };      // neither 0 nor kKeyForced
+    auto before = [&](const uint32_t *x) {                                  // what the waves before this one left
+        const uint32_t s = sel_scan(lane < W ? x[lane] : 0u);
+        return w ? sel_lane(s, w - 1) : 0u;
+    };
     // ---- how many are candidates, how many forced, which range the others span ----
-    uint32_t mn = 0xffffffffu, mx = 0, nv = 0, nf = 0;
+    uint32_t mnc = 0, mx = 0, nv = 0, nf = 0;                           // mnc: the complement of the smallest
     for (int sl = 0; sl < slabs; sl++) {
-        load(sl);
+        if (MULTI && sl > 0) fetch(sl, kr);
 #pragma unroll
         for (int i = 0; i < NR; i++) {
             const uint32_t k = kr[i];
-            nf += k == kKeyForced;
-            if (k != 0 && k != kKeyForced) { nv++; mn = min(mn, k); mx = max(mx, k); }
+            nf += (uint32_t)__popcll(__ballot(k == kKeyForced));
+            nv += (uint32_t)__popcll(__ballot(scored(k)));
+            if (scored(k)) { mnc = max(mnc, ~k); mx = max(mx, k); }
         }
     }
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        mn = min(mn, (uint32_t)__shfl_xor((int)mn, off));
-        mx = max(mx, (uint32_t)__shfl_xor((int)mx, off));
-        nv += (uint32_t)__shfl_xor((int)nv, off);
-        nf += (uint32_t)__shfl_xor((int)nf, off);
-    }
-    if (lane == 0) { red[0][w] = mn; red[1][w] = mx; red[2][w] = nv; red[3][w] = nf; }
+    mnc = sel_wave_max(mnc);
+    mx = sel_wave_max(mx);
+    if (lane == 0) { S.red[0][w] = mnc; S.red[1][w] = mx; S.red[2][w] = nv; S.red[3][w] = nf; }
+    for (int i = tid; i < BINS; i += THREADS) S.hist[i] = 0;
+    if (tid == 0) S.list_n = 0;
     __syncthreads();
-    nv = nf = 0;
-    for (int i = 0; i < W; i++) {
-        mn = min(mn, red[0][i]);
-        mx = max(mx, red[1][i]);
-        nv += red[2][i];
-        nf += red[3][i];
-    }
-    // chosen: keys above thr, and the first `ties` equal to it
+    mnc = sel_wave_max(lane < W ? S.red[0][lane] : 0u);
+    mx = sel_wave_max(lane < W ? S.red[1][lane] : 0u);
+    nv = sel_lane(sel_scan(lane < W ? S.red[2][lane] : 0u), W - 1);
+    nf = sel_lane(sel_scan(lane < W ? S.red[3][lane] : 0u), W - 1);
+    // chosen: keys above thr, and -- where not all of them fit -- the first `ties` equal to it
     uint32_t thr = 0, ties = 0;
-    const uint32_t want = (uint32_t)A.keep > nf ? (uint32_t)A.keep - nf : 0u;
+    const uint32_t want = (uint32_t)keep > nf ? (uint32_t)keep - nf : 0u;
     if (want == 0) {
         thr = kKeyForced - 1;
     } else if (nv > want) {
-        uint32_t base = mn, need = want, limit = mx - mn;                 // keys base .. base + limit are in question
+        uint32_t base = ~mnc, need = want, limit = mx - base;               // keys base .. base + limit are in question
         for (;;) {
-            const int bits = limit ? 32 - __builtin_clz(limit) : 0, shift = bits > 11 ? bits - 11 : 0;
-            for (int i = tid; i < kSelBins; i += THREADS) hist[i] = 0;
-            __syncthreads();
+            const int bits = limit ? 32 - __builtin_clz(limit) : 0, shift = bits > BIN_BITS ? bits - BIN_BITS : 0;
+            auto in_range = [&](uint32_t k) { return scored(k) && k >= base && k - base <= limit; };
             for (int sl = 0; sl < slabs; sl++) {
-                if (slabs > 1) load(sl);
+                if (MULTI) fetch(sl, kr);
 #pragma unroll
-                for (int i = 0; i < NR; i++) {
-                    const uint32_t k = kr[i];
-                    if (k != 0 && k != kKeyForced && k >= base && k - base <= limit) atomicAdd(&hist[(k - base) >> shift], 1u);
-                }
+                for (int i = 0; i < NR; i++)
+                    if (in_range(kr[i])) atomicAdd(&S.hist[(kr[i] - base) >> shift], 1u);
             }
             __syncthreads();
-            // counts of the bins above this thread's, from the top down
+            // thread tid owns BPT bins, counted from the top
             uint32_t own[BPT], sum = 0;
 #pragma unroll
-            for (int i = 0; i < BPT; i++) { own[i] = hist[tid * BPT + i]; sum += own[i]; }
-            uint32_t above = sum;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const uint32_t v = (uint32_t)__shfl_down((int)above, off);
-                if (lane + off < 64) above += v;
-            }
-            if (lane == 0) red[0][w] = above;
+            for (int i = 0; i < BPT; i++) { own[i] = S.hist[BINS - 1 - (tid * BPT + i)]; sum += own[i]; }
+            const uint32_t incl = sel_scan(sum);
+            if (lane == 63) S.above_w[w] = incl;
             __syncthreads();
-            above -= sum;
-            for (int i = w + 1; i < W; i++) above += red[0][i];
+            uint32_t above = incl - sum + before(S.above_w);
             if (above < need && need <= above + sum) {
-                uint32_t ab = above;
 #pragma unroll
-                for (int i = BPT - 1; i >= 0; i--) {
-                    if (ab < need && need <= ab + own[i]) { found[0] = (uint32_t)(tid * BPT + i); found[1] = need - ab; found[2] = own[i]; }
-                    ab += own[i];
+                for (int i = 0; i < BPT; i++) {
+                    if (above < need && need <= above + own[i]) {
+                        S.found[0] = (uint32_t)(BINS - 1 - (tid * BPT + i));
+                        S.found[1] = need - above;
+                        S.found[2] = own[i];
+                    }
+                    above += own[i];
                 }
             }
             __syncthreads();
-            base += found[0] << shift;
-            need = found[1];
-            if (found[2] == need) { thr = base - 1; break; }              // the whole bin
+            const uint32_t bin = S.found[0], in_bin = S.found[2];
+            need = S.found[1];
+            base += bin << shift;
+            if (in_bin == need) { thr = base - 1; break; }                  // the whole bin
             if (shift == 0) { thr = base; ties = need; break; }
-            limit = min((1u << shift) - 1, limit - (found[0] << shift));
+            limit = min((1u << shift) - 1, limit - (bin << shift));
+            if (in_bin <= kSelList) {
+                // few are left: every wave settles them by itself, counting for each how many are larger
+                for (int sl = 0; sl < slabs; sl++) {
+                    if (MULTI) fetch(sl, kr);
+                    uint32_t hits = 0;
+#pragma unroll
+                    for (int i = 0; i < NR; i++) hits |= in_range(kr[i]) ? 1u << i : 0u;
+                    if (hits) {
+                        uint32_t at = atomicAdd(&S.list_n, (uint32_t)__popc(hits));
+#pragma unroll
+                        for (int i = 0; i < NR; i++)
+                            if (hits >> i & 1) S.list[at++] = kr[i] - base;
+                    }
+                }
+                __syncthreads();
+                const uint32_t mine = S.list[min((uint32_t)lane, in_bin - 1)];
+                uint32_t larger = 0, equal = 0;
+                for (uint32_t i = 0; i < in_bin; i++) {
+                    const uint32_t o = sel_lane(mine, (int)i);
+                    larger += o > mine;
+                    equal += o == mine;
+                }
+                const uint64_t it = __ballot(larger < need && need <= larger + equal);        // lanes that hold the need-th largest
+                const int at = __builtin_ctzll(it);
+                thr = base + sel_lane(mine, at);
+                ties = need - sel_lane(larger, at);
+                if (ties == sel_lane(equal, at)) { thr--; ties = 0; }
+                break;
+            }
+            for (int i = tid; i < BINS; i += THREADS) S.hist[i] = 0;
             __syncthreads();
         }
     }
     // ---- the chosen ones, in ascending order ----
+    auto lower = [](uint64_t m) {                                           // set bits below this lane's
+#if defined(__HIP_DEVICE_COMPILE__)
+        return (uint32_t)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+#else
+        return (uint32_t)m;
+#endif
+    };
     uint32_t done_gt = 0, done_eq = 0;
-    const uint64_t below = (1ull << lane) - 1;
     for (int sl = 0; sl < slabs; sl++) {
-        if (slabs > 1) load(sl);
-        __syncthreads();
-        uint64_t mg[NR], me[NR];
+        if (MULTI) fetch(sl, kr);
+        if (MULTI && sl > 0) __syncthreads();                                        // the counts of the slab before have been read
+        uint32_t cg = 0, ce = 0;
 #pragma unroll
         for (int i = 0; i < NR; i++) {
-            mg[i] = __ballot(kr[i] > thr);
-            me[i] = ties ? __ballot(kr[i] == thr) : 0ull;
-            if (lane == 0) { cgt[i * W + w] = (uint32_t)__popcll(mg[i]); ceq[i * W + w] = (uint32_t)__popcll(me[i]); }
+            cg += (uint32_t)__popcll(__ballot(kr[i] > thr));
+            if (ties) ce += (uint32_t)__popcll(__ballot(kr[i] == thr));
         }
+        if (lane == 0) { S.chosen_w[0][w] = cg; S.chosen_w[1][w] = ce; }
         __syncthreads();
-        if (w == 0) {                                                     // exclusive prefix sums of NR * W counts
-            constexpr int E = (NR * W + 63) / 64;
-            uint32_t sg = 0, se = 0, vg[E], ve[E];
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                const int x = lane * E + i;
-                vg[i] = x < NR * W ? cgt[x] : 0u;
-                ve[i] = x < NR * W ? ceq[x] : 0u;
-                sg += vg[i];
-                se += ve[i];
-            }
-            uint32_t ig = sg, ie = se;
-#pragma unroll
-            for (int off = 1; off < 64; off <<= 1) {
-                const uint32_t a1 = (uint32_t)__shfl_up((int)ig, off), a2 = (uint32_t)__shfl_up((int)ie, off);
-                if (lane >= off) { ig += a1; ie += a2; }
-            }
-            if (lane == 63) { found[0] = ig; found[1] = ie; }
-            ig -= sg;
-            ie -= se;
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                const int x = lane * E + i;
-                if (x < NR * W) { cgt[x] = ig; ceq[x] = ie; }
-                ig += vg[i];
-                ie += ve[i];
-            }
-        }
-        __syncthreads();
+        const uint32_t sg = sel_scan(lane < W ? S.chosen_w[0][lane] : 0u), se = sel_scan(lane < W ? S.chosen_w[1][lane] : 0u);
+        uint32_t bg = done_gt + (w ? sel_lane(sg, w - 1) : 0u), be = done_eq + (w ? sel_lane(se, w - 1) : 0u);
+        done_gt += sel_lane(sg, W - 1);
+        done_eq += sel_lane(se, W - 1);
+        const int b0 = sl * SLAB + w * NR * 64 + lane;
 #pragma unroll
         for (int i = 0; i < NR; i++) {
-            const uint32_t bg = done_gt + cgt[i * W + w] + (uint32_t)__popcll(mg[i] & below);
-            const uint32_t be = done_eq + ceq[i * W + w] + (uint32_t)__popcll(me[i] & below);
-            const bool eq = (me[i] >> lane) & 1;
-            if ((((mg[i] >> lane) & 1) || (eq && be < ties))) {
-                const uint32_t at = bg + min(be, ties);
-                if (at < (uint32_t)A.keep) out[at] = sl * SLAB + i * THREADS + tid;
+            const uint64_t mg = __ballot(kr[i] > thr);
+            uint32_t at = bg + lower(mg);
+            bool take = kr[i] > thr;
+            if (ties) {
+                const uint64_t me = __ballot(kr[i] == thr);
+                const uint32_t rank = be + lower(me);
+                take = take || (kr[i] == thr && rank < ties);
+                at += min(rank, ties);
+                be += (uint32_t)__popcll(me);
             }
+            if (take && at < (uint32_t)keep) out[at] = b0 + i * 64;
+            bg += (uint32_t)__popcll(mg);
         }
-        done_gt += found[0];
-        done_eq += found[1];
     }
-    for (uint32_t i = done_gt + min(done_eq, ties) + tid; i < (uint32_t)A.keep; i += THREADS) out[i] = -1;
+    for (uint32_t i = done_gt + min(done_eq, ties) + tid; i < (uint32_t)keep; i += THREADS) out[i] = -1;
+}
+
+template <int THREADS, int NR, bool MULTI>
+__global__ __launch_bounds__(THREADS) void topk_kernel(SelArgs A, int KVH)
+{
+    constexpr int SLAB = NR * THREADS;
+    __shared__ TopkLds<THREADS> S;
+    const int tid = threadIdx.x;
+    const uint32_t *keys = A.keys + (size_t)blockIdx.x * A.key_stride;
+    uint32_t kr[NR];
+    const int b0 = (tid >> 6) * NR * 64 + (tid & 63);
+    // the first slab is requested before the row's length is known, and cut afterwards
+#pragma unroll
+    for (int i = 0; i < NR; i++) kr[i] = (unsigned)(b0 + i * 64) < A.key_stride ? keys[b0 + i * 64] : 0u;
+    const int nb = sel_blocks_of_row(A, blockIdx.x / KVH);
+#pragma unroll
+    for (int i = 0; i < NR; i++) kr[i] = b0 + i * 64 < nb ? kr[i] : 0u;
+    topk_run<THREADS, NR, MULTI>(S, kr, nb, A.keep, A.out + (size_t)blockIdx.x * A.keep, [&](int sl, uint32_t (&k)[NR]) {
+#pragma unroll
+        for (int i = 0; i < NR; i++) {
+            const int idx = sl * SLAB + b0 + i * 64;
+            k[i] = idx < nb ? keys[idx] : 0u;
+        }
+    });
+}
+
+// Scores and selection of one (row, kv head) in one workgroup, for contexts of few blocks: the keys stay in LDS.
+template <int D, int THREADS>
+__global__ __launch_bounds__(THREADS) void select_kernel(Lay a, SelArgs A)
+{
+    constexpr int W = THREADS / 64, NR = kSelFused / THREADS, KS = D / 32;
+    __shared__ TopkLds<THREADS> S;
+    __shared__ uint32_t key_lds[kSelFused];
+    const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int t = blockIdx.x / a.KVH, h = blockIdx.x - t * a.KVH, GQ = a.QH / a.KVH;
+    const int32_t *tab = A.tables + (size_t)t * A.table_stride;
+    const int nb = min(sel_blocks_of_row(A, t), kSelFused);
+    const int groups = (nb + 15) / 16;
+    int blk = w * 16 + c < nb ? tab[w * 16 + c] : -1;
+    sel_i32x4 qa[KS];
+    const int eq = sel_query<D>(A.q + ((size_t)t * a.QH + h * GQ + min(c & (A.P - 1), GQ - 1)) * D * 2, g, A.io_dtype, qa);
+    float qm[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) qm[j] = sel_pow2(__shfl(eq, 4 * g + j));
+    for (int gi = w; gi < groups; gi += W) {
+        const bool hole = blk < 0 || blk >= a.NB;
+        const size_t entry = (size_t)(hole ? 0 : blk) * a.KVH + h;          // block 0 is always mapped; its score is not used
+        const uint8_t *cp = A.bounds + entry * (2 * D) + g * 16;
+        uint4 bv[KS];
+#pragma unroll
+        for (int k = 0; k < KS; k++) bv[k] = *(const uint4 *)(cp + k * 64);
+        const int e = hole ? kNoBlock : (int)(int8_t)A.exps[entry], b = gi * 16 + c;
+        blk = b + W * 16 < nb ? tab[b + W * 16] : -1;
+        sel_i32x4 acc = {0, 0, 0, 0};
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[k], __builtin_bit_cast(sel_i32x4, bv[k]), acc, 0, 0, 0);
+#endif
+        const float x = sel_row_max(acc, qm, A.P, e == kNoBlock ? 0.0f : sel_pow2(e));
+        if (g == 0) key_lds[b] = sel_key_of(A, x, b, nb, e);
+    }
+    __syncthreads();
+    uint32_t kr[NR];
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+        const int b = (w * NR + i) * 64 + lane;
+        kr[i] = b < nb ? key_lds[b] : 0u;
+    }
+    topk_run<THREADS, NR, false>(S, kr, nb, A.keep, A.out + (size_t)blockIdx.x * A.keep, [](int, uint32_t (&)[NR]) {});
 }
 
 static unsigned sel_key_stride(const Lay &a, int max_seq_len)
@@ -318,12 +578,12 @@ static unsigned sel_key_stride(const Lay &a, int max_seq_len)
 }
 
 template <int D>
-static void launch_score(const Lay &a, const SelArgs &A, int sets, dim3 grid, hipStream_t st)
+static void launch_score(const Lay &a, const SelArgs &A, bool tile, dim3 grid, hipStream_t st)
 {
     if constexpr (D <= 256) {
-        if (sets == 4) { hipLaunchKernelGGL((score_kernel<D, 4>), grid, dim3(256), 0, st, a, A); return; }
+        if (tile) { hipLaunchKernelGGL((score_tile_kernel<D, 2>), grid, dim3(512), 0, st, a, A); return; }
     }
-    hipLaunchKernelGGL((score_kernel<D, 1>), grid, dim3(256), 0, st, a, A);
+    hipLaunchKernelGGL((score_kernel<D>), grid, dim3(256), 0, st, a, A);
 }
 
 } // namespace drk
@@ -369,28 +629,43 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
     A.table_stride = table_stride; A.pos_start = pos_start; A.T = T; A.max_seq_len = max_seq_len;
     A.keep = n_keep; A.sink = n_sink; A.recent = n_recent; A.io_dtype = io_dtype;
     A.bs_div = mk_div((unsigned)a.bs);
-    A.P = 1;
+    A.P = 4;
     while (A.P < a.QH / a.KVH) A.P *= 2;
-    A.R = table_stride == 0 ? 16 / A.P : 1;
-    const int sets = table_stride == 0 && a.D <= 256 && T > A.R ? 4 : 1;
+    A.R = table_stride == 0 && T > 1 ? 16 / A.P : 1;
+    const bool tile = table_stride == 0 && a.D <= 256 && T > 4 * A.R;      // more than four sets of rows over one table
     const int n = (int)(((size_t)max_seq_len + a.bs - 1) / a.bs);
     hipStream_t st = (hipStream_t)stream;
+    if (n <= kSelFused && a.D <= 256 && !tile) {
+        const dim3 grid(T * a.KVH);
+        if (a.D == 64) hipLaunchKernelGGL((select_kernel<64, 1024>), grid, dim3(1024), 0, st, a, A);
+        else if (a.D == 128) hipLaunchKernelGGL((select_kernel<128, 1024>), grid, dim3(1024), 0, st, a, A);
+        else hipLaunchKernelGGL((select_kernel<256, 512>), grid, dim3(512), 0, st, a, A);
+        DRK_LAUNCH_CHECK("select_kernel");
+        return DRK_OK;
+    }
     if (n > 0) {
-        const size_t tiles = ((size_t)T + A.R * sets - 1) / (A.R * sets), groups = ((size_t)n + 15) / 16;
-        if (tiles > 65535 || a.KVH > 65535) return fail(DRK_ERR_UNSUPPORTED, "block_select: %d rows are more than one launch takes", T);
+        const int rows = tile ? 16 * A.R : A.R;
+        const size_t tiles = ((size_t)T + rows - 1) / rows, groups = ((size_t)n + 15) / 16;
+        if (tiles > 65535 || groups > 65535) return fail(DRK_ERR_UNSUPPORTED, "block_select: %d rows are more than one launch takes", T);
         const size_t all = groups * a.KVH * tiles;                        // 16-block groups of every kv head and row tile
-        A.groups_per_wave = (int)(all / 4096 < 1 ? 1 : (all / 4096 > 16 ? 16 : all / 4096));
-        const dim3 grid((unsigned)((groups + 4 * A.groups_per_wave - 1) / (4 * A.groups_per_wave)), a.KVH, (unsigned)tiles);
+        const size_t units = tile ? kSelTileWgs : kSelWaves;              // as many as should have work of their own
+        const size_t gpw = (all + units - 1) / units;
+        A.groups_per_wave = (int)(gpw > 32 ? 32 : gpw);
+        if (tile) A.groups_per_wave = (int)((gpw + 1) & ~(size_t)1);
+        const size_t per = (size_t)A.groups_per_wave * (tile ? 1 : 4);
+        const dim3 grid(a.KVH, (unsigned)((groups + per - 1) / per), (unsigned)tiles);
         switch (a.D) {
-        case 64: launch_score<64>(a, A, sets, grid, st); break;
-        case 128: launch_score<128>(a, A, sets, grid, st); break;
-        case 256: launch_score<256>(a, A, sets, grid, st); break;
-        default: launch_score<512>(a, A, sets, grid, st); break;
+        case 64: launch_score<64>(a, A, tile, grid, st); break;
+        case 128: launch_score<128>(a, A, tile, grid, st); break;
+        case 256: launch_score<256>(a, A, tile, grid, st); break;
+        default: launch_score<512>(a, A, tile, grid, st); break;
         }
         DRK_LAUNCH_CHECK("score_kernel");
     }
-    if (n > 2048) hipLaunchKernelGGL((topk_kernel<1024>), dim3(T * a.KVH), dim3(1024), 0, st, A, a.KVH);
-    else hipLaunchKernelGGL((topk_kernel<256>), dim3(T * a.KVH), dim3(256), 0, st, A, a.KVH);
+    const dim3 rows(T * a.KVH);
+    if (n > 8192) hipLaunchKernelGGL((topk_kernel<1024, 8, true>), rows, dim3(1024), 0, st, A, a.KVH);
+    else if (n > 2048) hipLaunchKernelGGL((topk_kernel<1024, 8, false>), rows, dim3(1024), 0, st, A, a.KVH);
+    else hipLaunchKernelGGL((topk_kernel<256, 8, false>), rows, dim3(256), 0, st, A, a.KVH);
     DRK_LAUNCH_CHECK("topk_kernel");
     return DRK_OK;
 }

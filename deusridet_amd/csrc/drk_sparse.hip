@@ -3,7 +3,7 @@
 // The listed blocks' tokens are one long axis, cut into groups of 16 (a block is a whole number of
 // them).  A workgroup takes a piece of one (row, kv head)'s groups: first every thread turns a few
 // groups into descriptors in LDS -- list entry, block table, page offset: the dependent loads happen
-// there, side by side, and groups without a token drop out -- then its four waves walk them
+// there, side by side, and groups without a token drop out -- then its eight waves walk them
 // independently, each with a running maximum and sum per query head and the output in registers:
 //   S[token][head] = K[16 x D] Q^T       D/32 x v_mfma_f32_16x16x32
 //   O[head][dim]  += P[heads x 16] V     D/16 x v_mfma_f32_16x16x16
@@ -15,6 +15,7 @@ namespace drk {
 
 constexpr int kSpGroups = 512;          // 16-token groups one workgroup may own (descriptors in LDS)
 constexpr int kSpMaxPieces = 64;        // pieces of a row: a lane each in the merge
+constexpr int kSpWaves = 8;
 constexpr int kSpWgs = 512;             // workgroups a launch aims at: 2 per CU
 
 struct SparseArgs {
@@ -30,18 +31,21 @@ struct SparseArgs {
     float scale_log2e;
 };
 
-template <int DT, int D>
-__global__ __launch_bounds__(256, D == 128 ? 4 : 2) void sparse_kernel(SparseArgs A)
+template <int DT, int D, bool NT>
+__global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel(SparseArgs A)
 {
     using Geo = StreamGeo<DT, D>;
     [[maybe_unused]] constexpr bool Q8 = Geo::q8;
     constexpr int DOT = KvTraits<DT>::dot;
-    __shared__ __align__(16) uint8_t k_lds[4][16 * Geo::PITCH];
-    __shared__ __align__(16) float o_lds[4][4][D];
-    __shared__ float mw_lds[4][16], lw_lds[4][16];
+    constexpr int W = kSpWaves;
+    __shared__ __align__(16) uint8_t k_lds[W][16 * Geo::PITCH];   // the waves' staged keys; at the end their outputs
+    __shared__ __align__(16) uint8_t q_lds[16 * Geo::PITCH];
+    __shared__ float mw_lds[W][16], lw_lds[W][16];
     __shared__ uint32_t goff[kSpGroups], gsoff[DT == DRK_INT8 ? kSpGroups : 1];
     __shared__ uint8_t gcnt[kSpGroups];
-    __shared__ int wcount[4];
+    __shared__ int wcount[W];
+    static_assert(sizeof(k_lds) >= W * 4 * D * sizeof(float), "the waves' outputs of one round fit over the keys");
+    float (*o_lds)[4][D] = (float (*)[4][D]) & k_lds[0][0];
 
     const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -57,7 +61,7 @@ __global__ __launch_bounds__(256, D == 128 ? 4 : 2) void sparse_kernel(SparseArg
     const int32_t *tab = A.tables + (size_t)t * A.table_stride;
     const int g0 = piece * A.groups_per_piece, gn = min(A.groups_per_piece, A.groups - g0), gpb = A.bs / 16;
     int n = 0;
-    for (int i0 = 0; i0 < gn; i0 += 256) {
+    for (int i0 = 0; i0 < gn; i0 += W * 64) {
         const int gi = g0 + i0 + (int)threadIdx.x;
         uint32_t off = 0, soff = 0;
         int cnt = 0;
@@ -81,7 +85,8 @@ __global__ __launch_bounds__(256, D == 128 ? 4 : 2) void sparse_kernel(SparseArg
         if (lane == 0) wcount[w] = __popcll(live);
         __syncthreads();
         int at = n + __popcll(live & ((1ull << lane) - 1));
-        for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int i = 0; i < W; i++) {
             if (i < w) at += wcount[i];
             n += wcount[i];
         }
@@ -93,36 +98,37 @@ __global__ __launch_bounds__(256, D == 128 ? 4 : 2) void sparse_kernel(SparseArg
         __syncthreads();
     }
 
-    // ---- Q^T as the second operand: lane (head c, dims 32 kk + 8 g ..), heads GQ..15 are padding ----
-    uint4 qop[Geo::NQK];
+    // ---- the query heads as 16 rows in LDS, the second operand of the first product; rows GQ..15 are zero ----
+    for (int i = threadIdx.x; i < 16 * (D / 8); i += W * 64) {
+        const int r = i / (D / 8), ch = i - r * (D / 8);
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (r < GQ) v = *(const uint4 *)(A.q + (size_t)(bq + r) * (D * 2) + ch * 16);
+#if defined(__HIP_DEVICE_COMPILE__)
+        if (Q8 && A.io_dtype == DRK_BF16) {                  // quantised pages multiply in fp16
+            v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.x), bf16_hi(v.x)));
+            v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.y), bf16_hi(v.y)));
+            v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.z), bf16_hi(v.z)));
+            v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.w), bf16_hi(v.w)));
+        }
+#endif
+        *(uint4 *)(q_lds + r * Geo::PITCH + ch * 16) = v;
+    }
+    __syncthreads();
+    const uint8_t *const qrow = q_lds + c * Geo::PITCH + g * 16;
     float qbias = 0.0f;
-    {
+    if (DT == DRK_INT8) {                                     // sum of the head's query values, for the code offset
         float sq = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < Geo::NQK; kk++) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (c < GQ) v = *(const uint4 *)(A.q + (size_t)(bq + c) * (D * 2) + kk * 64 + g * 16);
-#if defined(__HIP_DEVICE_COMPILE__)
-            if (Q8 && A.io_dtype == DRK_BF16) {              // quantised pages multiply in fp16
-                v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.x), bf16_hi(v.x)));
-                v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.y), bf16_hi(v.y)));
-                v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.z), bf16_hi(v.z)));
-                v.w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.w), bf16_hi(v.w)));
-            }
-#endif
-            qop[kk] = v;
-            if (DT == DRK_INT8) {
-                sq = s_dot2<DOT>(v.x, kF16Ones, sq);
-                sq = s_dot2<DOT>(v.y, kF16Ones, sq);
-                sq = s_dot2<DOT>(v.z, kF16Ones, sq);
-                sq = s_dot2<DOT>(v.w, kF16Ones, sq);
-            }
+            const uint4 v = *(const uint4 *)(qrow + kk * 64);
+            sq = s_dot2<DOT>(v.x, kF16Ones, sq);
+            sq = s_dot2<DOT>(v.y, kF16Ones, sq);
+            sq = s_dot2<DOT>(v.z, kF16Ones, sq);
+            sq = s_dot2<DOT>(v.w, kF16Ones, sq);
         }
-        if (DT == DRK_INT8) {
-            sq += __shfl_xor(sq, 16);
-            sq += __shfl_xor(sq, 32);
-            qbias = kI8Bias * sq;
-        }
+        sq += __shfl_xor(sq, 16);
+        sq += __shfl_xor(sq, 32);
+        qbias = kI8Bias * sq;
     }
 
     w_f32x4 o[Geo::NPV];
@@ -141,13 +147,13 @@ __global__ __launch_bounds__(256, D == 128 ? 4 : 2) void sparse_kernel(SparseArg
     VRegs<DT, D> vreg = {};
     uint2 ksr = {}, vsr = {};
     if (w < n) {
-        kreg = load_k<DT, D>(A.pool_layer, goff[w], lane);
-        vreg = load_v<DT, D>(A.pool_layer, goff[w], A.kv_plane, lane);
+        kreg = load_k<DT, D, NT>(A.pool_layer, goff[w], lane);
+        vreg = load_v<DT, D, NT>(A.pool_layer, goff[w], A.kv_plane, lane);
         load_scales(w, ksr, vsr);
     }
-    for (int i = w; i < n; i += 4) {
+    for (int i = w; i < n; i += W) {
         const int lim = __builtin_amdgcn_readfirstlane((int)gcnt[i]);
-        const bool more = i + 4 < n;
+        const bool more = i + W < n;
         stage_k<DT, D>(klds, kreg, lane);
         float ks[4] = {1.0f, 1.0f, 1.0f, 1.0f}, vs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
         if (DT == DRK_INT8) {
@@ -158,19 +164,22 @@ __global__ __launch_bounds__(256, D == 128 ? 4 : 2) void sparse_kernel(SparseArg
         }
         uint32_t next = 0;
         if (more) {
-            next = goff[i + 4];
-            kreg = load_k<DT, D>(A.pool_layer, next, lane);
-            load_scales(i + 4, ksr, vsr);
+            next = goff[i + W];
+            kreg = load_k<DT, D, NT>(A.pool_layer, next, lane);
+            load_scales(i + W, ksr, vsr);
         }
         w_f32x4 sacc = {0.0f, 0.0f, 0.0f, 0.0f};
         const uint8_t *arow = klds + c * Geo::PITCH + g * 16;
 #pragma unroll
         for (int k0 = 0; k0 < Geo::NQK; k0 += 4) {
-            uint4 ka[4];
+            uint4 ka[4], qa[4];
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++) ka[kk] = *(const uint4 *)(arow + (k0 + kk) * 64);
+            for (int kk = 0; kk < 4; kk++) {
+                ka[kk] = *(const uint4 *)(arow + (k0 + kk) * 64);
+                qa[kk] = *(const uint4 *)(qrow + (k0 + kk) * 64);
+            }
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++) sacc = w_mfma_qk<DOT>(ka[kk], qop[k0 + kk], sacc);
+            for (int kk = 0; kk < 4; kk++) sacc = w_mfma_qk<DOT>(ka[kk], qa[kk], sacc);
         }
         // softmax of head c over tokens 4g..4g+3 (+ the other three lane groups)
         const int t0 = g * 4;
@@ -236,10 +245,10 @@ __global__ __launch_bounds__(256, D == 128 ? 4 : 2) void sparse_kernel(SparseArg
 #pragma unroll
             for (int e = 0; e < 8; e++) o[ch * 8 + e] = w_mfma_pv<DOT>(pa, vb[e], o[ch * 8 + e]);
         }
-        if (more) vreg = load_v<DT, D>(A.pool_layer, next, A.kv_plane, lane);
+        if (more) vreg = load_v<DT, D, NT>(A.pool_layer, next, A.kv_plane, lane);
     }
 
-    // ---- fold the four waves ----
+    // ---- fold the waves ----
     float lw = l_lane, psum = ps_lane;
     lw += __shfl_xor(lw, 16);
     lw += __shfl_xor(lw, 32);
@@ -248,17 +257,19 @@ __global__ __launch_bounds__(256, D == 128 ? 4 : 2) void sparse_kernel(SparseArg
         psum += __shfl_xor(psum, 32);
     }
     if (lane < 16) { mw_lds[w][lane] = m_run; lw_lds[w][lane] = lw; }
-    __syncthreads();
+    __syncthreads();                                          // (the staged keys have been read, too)
     float f_own[4], bias[4];                                  // this wave's weight / code offset for head 4g + j
 #pragma unroll
     for (int j = 0; j < 4; j++) {
         const int hh = 4 * g + j;
-        const float M = fmaxf(fmaxf(mw_lds[0][hh], mw_lds[1][hh]), fmaxf(mw_lds[2][hh], mw_lds[3][hh]));
+        float M = mw_lds[0][hh];
+#pragma unroll
+        for (int i = 1; i < W; i++) M = fmaxf(M, mw_lds[i][hh]);
         const float mo = mw_lds[w][hh];
         f_own[j] = mo == -INFINITY ? 0.0f : s_exp2(mo - M);
         bias[j] = DT == DRK_INT8 ? kI8Bias * __shfl(psum, hh) : 0.0f;
     }
-    for (int r = 0; r < (GQ + 3) >> 2; r++) {                 // 4 heads per round: head 4r + w is stored by wave w
+    for (int r = 0; r < (GQ + 3) >> 2; r++) {                 // 4 heads per round: wave w adds up half of head 4r + w / 2
         if (r > 0) __syncthreads();
         if (g == r) {
 #pragma unroll
@@ -274,25 +285,30 @@ __global__ __launch_bounds__(256, D == 128 ? 4 : 2) void sparse_kernel(SparseArg
                 }
         }
         __syncthreads();
-        const int hh = 4 * r + w;
+        const int hh = 4 * r + (w >> 1);
         if (hh >= GQ) continue;
-        const float M = fmaxf(fmaxf(mw_lds[0][hh], mw_lds[1][hh]), fmaxf(mw_lds[2][hh], mw_lds[3][hh]));
-        float L = 0.0f;
+        float M = mw_lds[0][hh], L = 0.0f;
 #pragma unroll
-        for (int ww = 0; ww < 4; ww++) {
-            const float ll = lw_lds[ww][hh];
-            if (ll != 0.0f) L = fmaf(ll, s_exp2(mw_lds[ww][hh] - M), L);      // (a NaN takes part)
+        for (int i = 1; i < W; i++) M = fmaxf(M, mw_lds[i][hh]);
+#pragma unroll
+        for (int i = 0; i < W; i++) {
+            const float ll = lw_lds[i][hh];
+            if (ll != 0.0f) L = fmaf(ll, s_exp2(mw_lds[i][hh] - M), L);       // (a NaN takes part)
         }
-        constexpr int VEC = D / 64;
-        const int d = lane * VEC;
+        constexpr int VEC = D / 128;                          // dims per lane
+        const int d = (w & 1) * (D / 2) + lane * VEC;
         float acc[VEC];
 #pragma unroll
-        for (int x = 0; x < VEC; x++) acc[x] = (o_lds[0][w][d + x] + o_lds[1][w][d + x]) + (o_lds[2][w][d + x] + o_lds[3][w][d + x]);
+        for (int x = 0; x < VEC; x++) {
+            acc[x] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < W; i++) acc[x] += o_lds[i][w >> 1][d + x];
+        }
         if (A.pieces > 1) {
             const size_t pi = (size_t)(bq + hh) * A.pieces + piece;
 #pragma unroll
             for (int x = 0; x < VEC; x++) A.part_o[pi * D + d + x] = acc[x];
-            if (lane == 0) { A.part_m[pi] = M; A.part_l[pi] = L; }
+            if (lane == 0 && !(w & 1)) { A.part_m[pi] = M; A.part_l[pi] = L; }
         } else if (L != 0.0f) {
             uint16_t *dst = A.out + (size_t)(bq + hh) * D + d;
             const uint16_t *gp = A.gate ? A.gate + (size_t)(bq + hh) * A.gate_stride + d : nullptr;
@@ -320,11 +336,21 @@ __global__ __launch_bounds__(64) void sparse_merge_kernel(SparseArgs A)
     if (__ballot(live) == 0) return;                           // no token took part
     const float wgt = live ? s_exp2(m - M) : 0.0f;
     const float L = s_wave_sum(live ? l * wgt : 0.0f);
-    float acc[VEC] = {};
-    for (int s = 0; s < A.pieces; s++) {
-        const float ws = s_lane(wgt, s);
+    typedef float fvec __attribute__((ext_vector_type(VEC)));
+    fvec acc = {};
+    for (int s0 = 0; s0 < A.pieces; s0 += 8) {                 // eight rows in flight
+        fvec o[8];
+        float ws[8];
 #pragma unroll
-        for (int x = 0; x < VEC; x++) acc[x] = fmaf(A.part_o[(base + s) * D + d + x], ws, acc[x]);
+        for (int u = 0; u < 8; u++) {
+            const int s = min(s0 + u, A.pieces - 1);
+            ws[u] = s0 + u < A.pieces ? s_lane(wgt, s) : 0.0f;
+            o[u] = *(const fvec *)(A.part_o + (base + s) * D + d);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+#pragma unroll
+            for (int x = 0; x < VEC; x++) acc[x] = fmaf(o[u][x], ws[u], acc[x]);
     }
     uint16_t *dst = A.out + row * D + d;
     const uint16_t *gp = A.gate ? A.gate + row * A.gate_stride + d : nullptr;
@@ -336,13 +362,13 @@ __global__ __launch_bounds__(64) void sparse_merge_kernel(SparseArgs A)
     }
 }
 
-// Pieces of a (row, kv head): enough workgroups for the chip, but no piece shorter than four groups (one per wave)
+// Pieces of a (row, kv head): enough workgroups for the chip, but no piece shorter than a group per wave
 // and none longer than the descriptor table.
 static int sparse_pieces(const Lay &a, int T, int n_keep, int *groups_per_piece)
 {
     const size_t groups = (size_t)n_keep * (a.bs / 16), rows = (size_t)T * a.KVH;
     size_t p = (kSpWgs + rows - 1) / rows;
-    p = p > (groups + 3) / 4 ? (groups + 3) / 4 : p;
+    p = p > (groups + kSpWaves - 1) / kSpWaves ? (groups + kSpWaves - 1) / kSpWaves : p;
     p = p > kSpMaxPieces ? kSpMaxPieces : p;
     const size_t least = (groups + kSpGroups - 1) / kSpGroups;
     p = p < least ? least : p;
@@ -425,10 +451,16 @@ int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void
     A.scale_log2e = scale * kSLog2e;
     hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)((size_t)T * A.pieces * a.KVH));
-#define DRK_SPARSE_LAUNCH(DT)                                                                              \
-    do {                                                                                                   \
-        if (a.D == 128) hipLaunchKernelGGL((sparse_kernel<DT, 128>), grid, dim3(256), 0, st, A);           \
-        else hipLaunchKernelGGL((sparse_kernel<DT, 256>), grid, dim3(256), 0, st, A);                      \
+    const bool shared = table_stride == 0 && T > 1;           // rows over one table meet in the same pages: keep them cached
+#define DRK_SPARSE_LAUNCH2(DT, D)                                                                                          \
+    do {                                                                                                                   \
+        if (shared) hipLaunchKernelGGL((sparse_kernel<DT, D, false>), grid, dim3(kSpWaves * 64), 0, st, A);                \
+        else hipLaunchKernelGGL((sparse_kernel<DT, D, true>), grid, dim3(kSpWaves * 64), 0, st, A);                        \
+    } while (0)
+#define DRK_SPARSE_LAUNCH(DT)                                                                                              \
+    do {                                                                                                                   \
+        if (a.D == 128) DRK_SPARSE_LAUNCH2(DT, 128);                                                                       \
+        else DRK_SPARSE_LAUNCH2(DT, 256);                                                                                  \
     } while (0)
     switch (a.dtype) {
     case DRK_F16: DRK_SPARSE_LAUNCH(DRK_F16); break;
@@ -437,6 +469,7 @@ int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void
     default: DRK_SPARSE_LAUNCH(DRK_FP8_E4M3); break;
     }
 #undef DRK_SPARSE_LAUNCH
+#undef DRK_SPARSE_LAUNCH2
     DRK_LAUNCH_CHECK("sparse_kernel");
     if (A.pieces > 1) {
         if (a.D == 128) hipLaunchKernelGGL((sparse_merge_kernel<128>), dim3(T * a.QH), dim3(64), 0, st, A);

@@ -99,14 +99,21 @@ template <int DT, int D> struct KRegs { uint4 r[StreamGeo<DT, D>::NK]; };
 // The 16-token run of one kv head at offset `off` of the layer, in units of 16 bytes (kNone:
 // the run has no page).  A missing run is loaded from offset 0 -- always mapped -- instead of being
 // predicated off: its K only feeds scores that are masked anyway, and its V is cleared
-// by the consumer where a stale bit pattern could matter.
-template <int DT, int D>
+// by the consumer where a stale bit pattern could matter.  NT: streaming loads, for pages one workgroup
+// reads; plain loads where several read the same ones.
+template <bool NT>
+__device__ __forceinline__ uint4 ld128(const void *p)
+{
+    if constexpr (NT) return ld_stream128(p);
+    return *(const uint4 *)p;
+}
+template <int DT, int D, bool NT = true>
 __device__ __forceinline__ KRegs<DT, D> load_k(const uint8_t *__restrict__ layer, uint32_t off, int lane)
 {
     KRegs<DT, D> k;
     const uint8_t *p = layer + ((size_t)(off == 0xffffffffu ? 0u : off) << 4) + (size_t)lane * 16;
 #pragma unroll
-    for (int j = 0; j < StreamGeo<DT, D>::NK; j++) k.r[j] = ld_stream128(p + 1024 * j);
+    for (int j = 0; j < StreamGeo<DT, D>::NK; j++) k.r[j] = ld128<NT>(p + 1024 * j);
     return k;
 }
 
@@ -179,7 +186,7 @@ __device__ __forceinline__ w_f32x4 w_mfma_pv(const uint2 &a, const uint2 &b, w_f
 template <int DT, int D, bool Q8 = KvTraits<DT>::q8> struct VRegs { uint4 r[4][StreamGeo<DT, D>::NCH]; };
 template <int DT, int D> struct VRegs<DT, D, true> { uint2 r[4][StreamGeo<DT, D>::NCH]; };
 
-template <int DT, int D>
+template <int DT, int D, bool NT = true>
 __device__ __forceinline__ VRegs<DT, D> load_v(const uint8_t *__restrict__ layer, uint32_t off, uint32_t kv_plane, int lane)
 {
     using G = StreamGeo<DT, D>;
@@ -189,8 +196,13 @@ __device__ __forceinline__ VRegs<DT, D> load_v(const uint8_t *__restrict__ layer
     for (int j = 0; j < 4; j++)
 #pragma unroll
         for (int ch = 0; ch < G::NCH; ch++) {
-            if constexpr (G::q8) v.r[j][ch] = ld_stream64(p + j * G::RB + ch * 128 + (lane & 15) * 8);
-            else v.r[j][ch] = ld_stream128(p + j * G::RB + ch * 256 + (lane & 15) * 16);
+            if constexpr (G::q8) {
+                const uint8_t *at = p + j * G::RB + ch * 128 + (lane & 15) * 8;
+                if constexpr (NT) v.r[j][ch] = ld_stream64(at);
+                else v.r[j][ch] = *(const uint2 *)at;
+            } else {
+                v.r[j][ch] = ld128<NT>(p + j * G::RB + ch * 256 + (lane & 15) * 16);
+            }
         }
     return v;
 }

@@ -1,10 +1,11 @@
 // drk_sparse.hip -- paged GQA attention over the blocks a selection lists for each (row, kv head).
 //
 // The listed blocks' tokens are one long axis, cut into groups of 16 (a block is a whole number of
-// them).  A workgroup takes a piece of one (row, kv head)'s groups: first every thread turns a few
-// groups into descriptors in LDS -- list entry, block table, page offset: the dependent loads happen
-// there, side by side, and groups without a token drop out -- then its eight waves walk them
-// independently, each with a running maximum and sum per query head and the output in registers:
+// them).  A workgroup of eight waves takes a piece of one (row, kv head)'s groups -- or, where rows abound, two,
+// four or eight whole rows: first every thread turns a few groups into descriptors in LDS -- list entry, block
+// table, page offset: the dependent loads happen there, side by side, and groups without a token drop
+// out -- then the waves walk them independently, each with a running maximum and sum per query head and the
+// output in registers:
 //   S[token][head] = K[16 x D] Q^T       D/32 x v_mfma_f32_16x16x32
 //   O[head][dim]  += P[heads x 16] V     D/16 x v_mfma_f32_16x16x16
 // with the query heads of the group as the 16-wide operand.  The waves' states meet at the end; a row
@@ -25,49 +26,80 @@ struct SparseArgs {
     uint16_t *out;
     float *part_o, *part_m, *part_l;     // [T][QH][pieces]([D])
     size_t gate_stride;
-    int table_stride, pos_start, KVH, QH, NB, bs, keep, io_dtype;
+    int table_stride, pos_start, T, KVH, QH, NB, bs, keep, io_dtype;
     int pieces, groups_per_piece, groups;    // 16-token groups of a (row, kv head)'s list
     unsigned head_stride, kv_plane, block_stride, scale_plane, row_bytes;
     float scale_log2e;
 };
 
-template <int DT, int D, bool NT>
+// what a workgroup keeps in LDS beside the staged keys: the rows' query heads and group descriptors
+struct SparseLds {
+    unsigned q, desc, total;             // bytes per row of queries / of descriptors (offsets, scale offsets, counts), all
+    unsigned soff, cnt;                  // where they begin inside a row's descriptors
+};
+__host__ __device__ inline SparseLds sparse_lds(int GQ, int pitch, int groups, bool scales, int rows)
+{
+    SparseLds s;
+    s.q = (unsigned)(GQ * pitch);
+    s.soff = (unsigned)groups * 4;
+    s.cnt = s.soff * (scales ? 2 : 1);
+    s.desc = (s.cnt + (unsigned)groups + 15) & ~15u;
+    s.total = (s.q + s.desc) * (unsigned)rows;
+    return s;
+}
+
+// WPR waves per row.  More than one: a row's waves take every WPR-th group and fold their states at the end.
+template <int DT, int D, bool NT, int WPR>
 __global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel(SparseArgs A)
 {
     using Geo = StreamGeo<DT, D>;
     [[maybe_unused]] constexpr bool Q8 = Geo::q8;
     constexpr int DOT = KvTraits<DT>::dot;
-    constexpr int W = kSpWaves;
-    __shared__ __align__(16) uint8_t k_lds[W][16 * Geo::PITCH];   // the waves' staged keys; at the end their outputs
-    __shared__ __align__(16) uint8_t q_lds[16 * Geo::PITCH];
-    __shared__ float mw_lds[W][16], lw_lds[W][16];
-    __shared__ uint32_t goff[kSpGroups], gsoff[DT == DRK_INT8 ? kSpGroups : 1];
-    __shared__ uint8_t gcnt[kSpGroups];
-    __shared__ int wcount[W];
-    static_assert(sizeof(k_lds) >= W * 4 * D * sizeof(float), "the waves' outputs of one round fit over the keys");
-    float (*o_lds)[4][D] = (float (*)[4][D]) & k_lds[0][0];
+    constexpr int W = WPR, ROWS = kSpWaves / WPR, RT = WPR * 64;      // RT: threads per row
+    __shared__ __align__(16) uint8_t k_lds[kSpWaves][16 * Geo::PITCH];   // the waves' staged keys; at the end their outputs
+    __shared__ float mw_all[kSpWaves][16], lw_all[kSpWaves][16];
+    __shared__ int wcount[kSpWaves];
+    extern __shared__ __align__(16) uint8_t dyn_lds[];
+    static_assert(sizeof(k_lds) >= kSpWaves * 4 * D * sizeof(float), "the waves' outputs of one round fit over the keys");
 
-    const int w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int rw = wave / WPR, w = wave - rw * WPR;                   // row of the workgroup, wave of the row
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15, rtid = w * 64 + lane;
     const int GQ = A.QH / A.KVH;
     // kv heads vary fastest: neighbouring workgroups, on different XCDs, read different heads' rows
     const int h = (int)(blockIdx.x % (unsigned)A.KVH), tp = (int)(blockIdx.x / (unsigned)A.KVH);
-    const int t = tp / A.pieces, piece = tp - t * A.pieces;
-    const int len = A.seq_lens ? A.seq_lens[t] : A.pos_start + t + 1;
+    const int t = (tp / A.pieces) * ROWS + rw, piece = tp - (tp / A.pieces) * A.pieces;
+    const bool row_on = t < A.T;
+    const int len = row_on ? (A.seq_lens ? A.seq_lens[t] : A.pos_start + t + 1) : 0;
     const int bq = t * A.QH + h * GQ;
+    const SparseLds S = sparse_lds(GQ, Geo::PITCH, A.groups_per_piece, DT == DRK_INT8, ROWS);
+    uint8_t *const q_lds = dyn_lds + rw * S.q, *const desc = dyn_lds + ROWS * S.q + rw * S.desc;
+    uint32_t *const goff = (uint32_t *)desc, *const gsoff = (uint32_t *)(desc + S.soff);
+    uint8_t *const gcnt = desc + S.cnt;
+    float (*const mw_lds)[16] = mw_all + rw * WPR, (*const lw_lds)[16] = lw_all + rw * WPR;
+    float (*const o_lds)[4][D] = (float (*)[4][D]) & k_lds[0][0] + rw * WPR;
+
+    // ---- the query heads, on their way while the descriptors are built ----
+    constexpr int QL = (16 * (D / 8) + RT - 1) / RT;                  // at most 16 heads of 16-byte chunks
+    uint4 qv[QL];
+    const int qn = row_on ? GQ * (D / 8) : 0;
+    const uint8_t *const qsrc = A.q + (size_t)(row_on ? bq : 0) * (D * 2);
+#pragma unroll
+    for (int i = 0; i < QL; i++)
+        if (rtid + i * RT < qn) qv[i] = *(const uint4 *)(qsrc + (size_t)(rtid + i * RT) * 16);
 
     // ---- descriptors of the groups that hold tokens, in order ----
     const int32_t *sel = A.sel + ((size_t)t * A.KVH + h) * A.keep;
     const int32_t *tab = A.tables + (size_t)t * A.table_stride;
     const int g0 = piece * A.groups_per_piece, gn = min(A.groups_per_piece, A.groups - g0), gpb = A.bs / 16;
     int n = 0;
-    for (int i0 = 0; i0 < gn; i0 += W * 64) {
-        const int gi = g0 + i0 + (int)threadIdx.x;
+    for (int i0 = 0; i0 < gn; i0 += RT) {
+        const int gi = g0 + i0 + rtid;
         uint32_t off = 0, soff = 0;
         int cnt = 0;
-        if (i0 + (int)threadIdx.x < gn) {
+        if (i0 + rtid < gn && len > 0) {
             const int e = gi / gpb, lb = sel[e], p0 = (gi - e * gpb) * 16;
-            if (lb >= 0 && lb <= (len - 1) / A.bs && len > 0) {
+            if (lb >= 0 && lb <= (len - 1) / A.bs) {
                 cnt = min(16, len - lb * A.bs - p0);
                 if (cnt > 0) {
                     const int blk = tab[lb];
@@ -82,29 +114,33 @@ __global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel
             }
         }
         const uint64_t live = __ballot(cnt > 0);
-        if (lane == 0) wcount[w] = __popcll(live);
-        __syncthreads();
         int at = n + __popcll(live & ((1ull << lane) - 1));
+        if constexpr (WPR > 1) {
+            if (lane == 0) wcount[wave] = __popcll(live);
+            __syncthreads();
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            if (i < w) at += wcount[i];
-            n += wcount[i];
+            for (int i = 0; i < W; i++) {
+                if (i < w) at += wcount[rw * WPR + i];
+                n += wcount[rw * WPR + i];
+            }
+        } else {
+            n += __popcll(live);
         }
         if (cnt > 0) {
             goff[at] = off;
             gcnt[at] = (uint8_t)cnt;
             if (DT == DRK_INT8) gsoff[at] = soff;
         }
-        __syncthreads();
+        if (WPR > 1) __syncthreads();                                 // the counts have been read
     }
 
-    // ---- the query heads as 16 rows in LDS, the second operand of the first product; rows GQ..15 are zero ----
-    for (int i = threadIdx.x; i < 16 * (D / 8); i += W * 64) {
-        const int r = i / (D / 8), ch = i - r * (D / 8);
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (r < GQ) v = *(const uint4 *)(A.q + (size_t)(bq + r) * (D * 2) + ch * 16);
+#pragma unroll
+    for (int i = 0; i < QL; i++) {
+        const int x = rtid + i * RT, r = x / (D / 8), ch = x - r * (D / 8);
+        if (x >= qn) continue;
+        uint4 v = qv[i];
 #if defined(__HIP_DEVICE_COMPILE__)
-        if (Q8 && A.io_dtype == DRK_BF16) {                  // quantised pages multiply in fp16
+        if (Q8 && A.io_dtype == DRK_BF16) {                           // quantised pages multiply in fp16
             v.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.x), bf16_hi(v.x)));
             v.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.y), bf16_hi(v.y)));
             v.z = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(bf16_lo(v.z), bf16_hi(v.z)));
@@ -114,9 +150,10 @@ __global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel
         *(uint4 *)(q_lds + r * Geo::PITCH + ch * 16) = v;
     }
     __syncthreads();
-    const uint8_t *const qrow = q_lds + c * Geo::PITCH + g * 16;
+    // operand rows GQ .. 15 repeat the last head: what comes out of them is not used
+    const uint8_t *const qrow = q_lds + min(c, GQ - 1) * Geo::PITCH + g * 16;
     float qbias = 0.0f;
-    if (DT == DRK_INT8) {                                     // sum of the head's query values, for the code offset
+    if (DT == DRK_INT8) {                                             // sum of the head's query values, for the code offset
         float sq = 0.0f;
 #pragma unroll
         for (int kk = 0; kk < Geo::NQK; kk++) {
@@ -135,10 +172,10 @@ __global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel
 #pragma unroll
     for (int e = 0; e < Geo::NPV; e++) o[e] = w_f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = -INFINITY, l_lane = 0.0f, ps_lane = 0.0f;
-    uint8_t *const klds = &k_lds[w][0];
+    uint8_t *const klds = &k_lds[wave][0];
     auto load_scales = [&](int i, uint2 &ks, uint2 &vs) {
         if (DT != DRK_INT8) return;
-        const uint8_t *p = A.pool_layer + ((size_t)gsoff[DT == DRK_INT8 ? i : 0] << 4) + g * 8;
+        const uint8_t *p = A.pool_layer + ((size_t)gsoff[i] << 4) + g * 8;
         ks = *(const uint2 *)p;
         vs = *(const uint2 *)(p + A.scale_plane);
     };
@@ -248,13 +285,40 @@ __global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel
         if (more) vreg = load_v<DT, D, NT>(A.pool_layer, next, A.kv_plane, lane);
     }
 
-    // ---- fold the waves ----
+    // ---- the end: fold the waves ----
     float lw = l_lane, psum = ps_lane;
     lw += __shfl_xor(lw, 16);
     lw += __shfl_xor(lw, 32);
     if (DT == DRK_INT8) {
         psum += __shfl_xor(psum, 16);
         psum += __shfl_xor(psum, 32);
+    }
+    if constexpr (WPR == 1) {
+        // nothing to fold: head 4g + j, dims ch * 128 + 8c .. + 7 are in this lane
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int hh = 4 * g + j;
+            const float L = __shfl(lw, hh), bias = DT == DRK_INT8 ? kI8Bias * __shfl(psum, hh) : 0.0f;
+            if (hh >= GQ || !row_on || L == 0.0f) continue;
+#pragma unroll
+            for (int ch = 0; ch < Geo::NCH; ch++) {
+                const int d = ch * 128 + c * 8;
+                const uint16_t *gp = A.gate ? A.gate + (size_t)(bq + hh) * A.gate_stride + d : nullptr;
+                uint4 gv = make_uint4(0u, 0u, 0u, 0u);
+                if (gp) gv = *(const uint4 *)gp;
+                const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w};
+                uint32_t y[4];
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    float v = (o[ch * 8 + e][j] - bias) / L;
+                    if (gp) v = sigmoid_gate_value(v, elem16_to_f((uint16_t)(gw[e >> 1] >> (16 * (e & 1))), A.io_dtype));
+                    const uint32_t b16 = f_to_elem16(v, A.io_dtype);
+                    y[e >> 1] = e & 1 ? y[e >> 1] | b16 << 16 : b16;
+                }
+                *(uint4 *)(A.out + (size_t)(bq + hh) * D + d) = make_uint4(y[0], y[1], y[2], y[3]);
+            }
+        }
+        return;
     }
     if (lane < 16) { mw_lds[w][lane] = m_run; lw_lds[w][lane] = lw; }
     __syncthreads();                                          // (the staged keys have been read, too)
@@ -269,7 +333,9 @@ __global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel
         f_own[j] = mo == -INFINITY ? 0.0f : s_exp2(mo - M);
         bias[j] = DT == DRK_INT8 ? kI8Bias * __shfl(psum, hh) : 0.0f;
     }
-    for (int r = 0; r < (GQ + 3) >> 2; r++) {                 // 4 heads per round: wave w adds up half of head 4r + w / 2
+    // 4 heads per round, whose dims the row's threads share out
+    constexpr int VEC = D / 128, UNITS = 4 * (D / VEC) / RT;  // dims per thread at a time, times per round
+    for (int r = 0; r < (GQ + 3) >> 2; r++) {
         if (r > 0) __syncthreads();
         if (g == r) {
 #pragma unroll
@@ -285,38 +351,39 @@ __global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel
                 }
         }
         __syncthreads();
-        const int hh = 4 * r + (w >> 1);
-        if (hh >= GQ) continue;
-        float M = mw_lds[0][hh], L = 0.0f;
 #pragma unroll
-        for (int i = 1; i < W; i++) M = fmaxf(M, mw_lds[i][hh]);
+        for (int u = 0; u < UNITS; u++) {
+            const int x = rtid + u * RT, hr = x / (D / VEC), hh = 4 * r + hr, d = (x - hr * (D / VEC)) * VEC;
+            if (hh >= GQ || !row_on) continue;
+            float M = mw_lds[0][hh], L = 0.0f;
 #pragma unroll
-        for (int i = 0; i < W; i++) {
-            const float ll = lw_lds[i][hh];
-            if (ll != 0.0f) L = fmaf(ll, s_exp2(mw_lds[i][hh] - M), L);       // (a NaN takes part)
-        }
-        constexpr int VEC = D / 128;                          // dims per lane
-        const int d = (w & 1) * (D / 2) + lane * VEC;
-        float acc[VEC];
+            for (int i = 1; i < W; i++) M = fmaxf(M, mw_lds[i][hh]);
 #pragma unroll
-        for (int x = 0; x < VEC; x++) {
-            acc[x] = 0.0f;
+            for (int i = 0; i < W; i++) {
+                const float ll = lw_lds[i][hh];
+                if (ll != 0.0f) L = fmaf(ll, s_exp2(mw_lds[i][hh] - M), L);   // (a NaN takes part)
+            }
+            float acc[VEC];
 #pragma unroll
-            for (int i = 0; i < W; i++) acc[x] += o_lds[i][w >> 1][d + x];
-        }
-        if (A.pieces > 1) {
-            const size_t pi = (size_t)(bq + hh) * A.pieces + piece;
+            for (int e = 0; e < VEC; e++) {
+                acc[e] = 0.0f;
 #pragma unroll
-            for (int x = 0; x < VEC; x++) A.part_o[pi * D + d + x] = acc[x];
-            if (lane == 0 && !(w & 1)) { A.part_m[pi] = M; A.part_l[pi] = L; }
-        } else if (L != 0.0f) {
-            uint16_t *dst = A.out + (size_t)(bq + hh) * D + d;
-            const uint16_t *gp = A.gate ? A.gate + (size_t)(bq + hh) * A.gate_stride + d : nullptr;
+                for (int i = 0; i < W; i++) acc[e] += o_lds[i][hr][d + e];
+            }
+            if (A.pieces > 1) {
+                const size_t pi = (size_t)(bq + hh) * A.pieces + piece;
 #pragma unroll
-            for (int x = 0; x < VEC; x++) {
-                float y = acc[x] / L;
-                if (gp) y = sigmoid_gate_value(y, elem16_to_f(gp[x], A.io_dtype));
-                dst[x] = f_to_elem16(y, A.io_dtype);
+                for (int e = 0; e < VEC; e++) A.part_o[pi * D + d + e] = acc[e];
+                if (d == 0) { A.part_m[pi] = M; A.part_l[pi] = L; }
+            } else if (L != 0.0f) {
+                uint16_t *dst = A.out + (size_t)(bq + hh) * D + d;
+                const uint16_t *gp = A.gate ? A.gate + (size_t)(bq + hh) * A.gate_stride + d : nullptr;
+#pragma unroll
+                for (int e = 0; e < VEC; e++) {
+                    float y = acc[e] / L;
+                    if (gp) y = sigmoid_gate_value(y, elem16_to_f(gp[e], A.io_dtype));
+                    dst[e] = f_to_elem16(y, A.io_dtype);
+                }
             }
         }
     }
@@ -375,6 +442,15 @@ static int sparse_pieces(const Lay &a, int T, int n_keep, int *groups_per_piece)
     if (p > kSpMaxPieces) return 0;
     *groups_per_piece = (int)((groups + p - 1) / p);
     return (int)((groups + *groups_per_piece - 1) / *groups_per_piece);
+}
+
+// Waves per row: as few as still give the chip the waves it holds (16 per CU at head_dim 128, 8 at 256).
+static int sparse_waves_per_row(const Lay &a, int T)
+{
+    const size_t rows = (size_t)T * a.KVH, waves = a.D == 128 ? 4096 : 2048;
+    int w = 8;
+    while (w > 1 && rows * (w / 2) >= waves) w /= 2;
+    return w;
 }
 
 static int sparse_check(const drk_kv_layout *g, Lay *a, int T, int n_keep, int *pieces, int *gpp, const char *who)
@@ -444,23 +520,34 @@ int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void
     A.gate = (const uint16_t *)gate; A.gate_stride = gate_stride; A.out = (uint16_t *)out;
     const size_t np = (size_t)T * a.QH * A.pieces;
     A.part_o = (float *)workspace; A.part_m = A.part_o + np * a.D; A.part_l = A.part_m + np;
-    A.table_stride = table_stride; A.pos_start = pos_start; A.KVH = a.KVH; A.QH = a.QH; A.NB = a.NB; A.bs = a.bs;
+    A.table_stride = table_stride; A.pos_start = pos_start; A.T = T; A.KVH = a.KVH; A.QH = a.QH; A.NB = a.NB; A.bs = a.bs;
     A.keep = n_keep; A.io_dtype = io_dtype; A.groups = n_keep * (a.bs / 16);
     A.head_stride = a.head_stride; A.kv_plane = a.kv_plane; A.block_stride = a.block_stride; A.scale_plane = a.scale_plane;
     A.row_bytes = a.row_bytes;
     A.scale_log2e = scale * kSLog2e;
     hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)((size_t)T * A.pieces * a.KVH));
     const bool shared = table_stride == 0 && T > 1;           // rows over one table meet in the same pages: keep them cached
-#define DRK_SPARSE_LAUNCH2(DT, D)                                                                                          \
-    do {                                                                                                                   \
-        if (shared) hipLaunchKernelGGL((sparse_kernel<DT, D, false>), grid, dim3(kSpWaves * 64), 0, st, A);                \
-        else hipLaunchKernelGGL((sparse_kernel<DT, D, true>), grid, dim3(kSpWaves * 64), 0, st, A);                        \
+    const int wpr = A.pieces > 1 ? 8 : sparse_waves_per_row(a, T);
+    const dim3 grid((unsigned)(((size_t)T * wpr + 7) / 8 * A.pieces * a.KVH));
+#define DRK_SPARSE_LAUNCH4(DT, D, NT, WPR)                                                                                  \
+    hipLaunchKernelGGL((sparse_kernel<DT, D, NT, WPR>), grid, dim3(kSpWaves * 64),                                          \
+                       sparse_lds(a.QH / a.KVH, StreamGeo<DT, D>::PITCH, A.groups_per_piece, DT == DRK_INT8, 8 / WPR).total, st, A)
+#define DRK_SPARSE_LAUNCH3(DT, D, NT)                                                                                       \
+    do {                                                                                                                    \
+        if (wpr == 8) DRK_SPARSE_LAUNCH4(DT, D, NT, 8);                                                                     \
+        else if (wpr == 4) DRK_SPARSE_LAUNCH4(DT, D, NT, 4);                                                                \
+        else if (wpr == 2) DRK_SPARSE_LAUNCH4(DT, D, NT, 2);                                                                \
+        else DRK_SPARSE_LAUNCH4(DT, D, NT, 1);                                                                              \
     } while (0)
-#define DRK_SPARSE_LAUNCH(DT)                                                                                              \
-    do {                                                                                                                   \
-        if (a.D == 128) DRK_SPARSE_LAUNCH2(DT, 128);                                                                       \
-        else DRK_SPARSE_LAUNCH2(DT, 256);                                                                                  \
+#define DRK_SPARSE_LAUNCH2(DT, D)                                                                                           \
+    do {                                                                                                                    \
+        if (shared) DRK_SPARSE_LAUNCH3(DT, D, false);                                                                       \
+        else DRK_SPARSE_LAUNCH3(DT, D, true);                                                                               \
+    } while (0)
+#define DRK_SPARSE_LAUNCH(DT)                                                                                               \
+    do {                                                                                                                    \
+        if (a.D == 128) DRK_SPARSE_LAUNCH2(DT, 128);                                                                        \
+        else DRK_SPARSE_LAUNCH2(DT, 256);                                                                                   \
     } while (0)
     switch (a.dtype) {
     case DRK_F16: DRK_SPARSE_LAUNCH(DRK_F16); break;
@@ -470,6 +557,8 @@ int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void
     }
 #undef DRK_SPARSE_LAUNCH
 #undef DRK_SPARSE_LAUNCH2
+#undef DRK_SPARSE_LAUNCH3
+#undef DRK_SPARSE_LAUNCH4
     DRK_LAUNCH_CHECK("sparse_kernel");
     if (A.pieces > 1) {
         if (a.D == 128) hipLaunchKernelGGL((sparse_merge_kernel<128>), dim3(T * a.QH), dim3(64), 0, st, A);

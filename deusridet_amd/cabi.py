@@ -243,9 +243,18 @@ def check(code):
     return code
 
 
+_functions = {}
+
+
 def call(name, *args):
     """Call an int-returning entry point and raise DrkError on failure."""
-    return check(getattr(lib(), name)(*args))
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(lib(), name)
+    code = fn(*args)
+    if code != OK:
+        check(code)
+    return code
 
 
 # ---- plumbing for callers that keep device memory in torch tensors -------------------

@@ -83,10 +83,7 @@ bool KvStream::init(CacheManager& cm, int max_context_len, ImportanceScorer* sco
 
 void KvStream::destroy()
 {
-    if (graph_) {
-        drk_graph_destroy(graph_);
-        graph_ = nullptr;
-    }
+    drop_graph();
     scorer_ = nullptr;                            // borrowed, and possibly gone already: its rows are not cleared here
     if (cm_) close_branches();
     if (d_pos_) drk_dev_free(d_pos_);
@@ -106,6 +103,7 @@ void KvStream::destroy()
         ev_attn_ = ev_mass_ = nullptr;
         mass_pending_ = false;
     }
+    drop_sparse();
     if (ws_decode_.ptr() || ws_prefill_.ptr()) {
         drk_device_synchronize();                 // launches that use the partials may still be running
         ws_decode_.release();
@@ -155,6 +153,9 @@ void KvStream::prefill_layer(int fa_layer_idx, const KvLayerIO& io, int M, hipSt
     paged_qk_norm_rope_write_batch(io.qg, io.k, io.v, io.q_norm, io.k_norm, io.q_scratch, pool.pool_ptr(),
                                    cm_->d_block_table(0), fa_layer_idx, current_pos_, M, pool.max_blocks(),
                                    pool.block_size(), d_rope_table_, table_positions_, stream);
+    if (d_bounds_)
+        paged_kv_bounds_update_batch(d_bounds_, pool.pool_ptr(), cm_->d_block_table(0), fa_layer_idx, 1, current_pos_, M,
+                                     pool.max_blocks(), pool.block_size(), stream);
     if (!scored) {
         paged_prefill_attention_gated(ws_prefill_, io.q_scratch, pool.pool_ptr(), cm_->d_block_table(0), io.qg + hd, 2 * hd, io.attn_out,
                                       fa_layer_idx, current_pos_, M, pool.max_blocks(), pool.block_size(), scale, stream);
@@ -233,11 +234,72 @@ int KvStream::set_branch_count(int n)
     positions_on_device_ = false;
     shared_tokens_ = branches_.empty() ? 0 : cm_->common_prefix_tokens(branches_.data(), (int)branches_.size());
     find_shared_groups();
-    if (graph_) {                        // a captured step is tied to the branch set it was recorded for
-        drk_graph_destroy(graph_);
-        graph_ = nullptr;
-    }
+    drop_graph();                        // a captured step is tied to the branch set it was recorded for
     return (int)branches_.size();
+}
+
+void KvStream::drop_graph()
+{
+    if (graph_) drk_graph_destroy(graph_);
+    graph_ = nullptr;
+}
+
+void KvStream::drop_sparse()
+{
+    if (!d_bounds_) return;
+    drk_device_synchronize();                                 // launches that use the buffers may still be running
+    drk_dev_free(d_bounds_);
+    ws_sparse_.release();
+    d_bounds_ = nullptr;
+    d_selected_ = nullptr;
+    sparse_keep_ = 0;
+}
+
+bool KvStream::set_sparse_decode(int min_tokens, int n_keep, int n_sink, int n_recent, hipStream_t stream)
+{
+    if (!cm_) return false;
+    if (n_keep == 0) {
+        if (d_bounds_) drop_graph();
+        drop_sparse();
+        return true;
+    }
+    const BlockPool& pool = cm_->block_pool();
+    const int bs = pool.block_size(), nb = pool.max_blocks();
+    if (min_tokens < 0 || n_keep < 0 || n_sink < 0 || n_recent < 0 || n_sink > n_keep || n_recent > n_keep - n_sink ||
+        !paged_sparse_attention_supported(bs) || (scorer_ && scorer_->d_new_scores()) || cm_->has_overflow_tier()) {
+        LOG_ERROR("Conscientia", "KvStream: decode over selected blocks (keep %d, %d first, %d last) is not possible here", n_keep, n_sink,
+                  n_recent);
+        return false;
+    }
+    const size_t bounds = paged_kv_bounds_bytes(nb, bs);
+    const size_t selected = (size_t)cm_->max_branches() * ModelConfig::NUM_KV_HEADS * n_keep * sizeof(int);
+    const size_t work = paged_sparse_workspace_bytes(cm_->max_branches(), max_context_len_, n_keep, nb, bs);
+    AttentionWorkspace fresh;
+    void* p = nullptr;
+    if (work == 0 || !fresh.reserve(work) || drk_dev_malloc(&p, bounds + selected) != DRK_OK) {
+        LOG_ERROR("Conscientia", "KvStream: buffers of the block selection: %s", drk_last_error());
+        return false;                                         // fresh frees itself
+    }
+    drop_graph();
+    drop_sparse();
+    ws_sparse_.adopt(fresh);
+    d_bounds_ = p;
+    d_selected_ = reinterpret_cast<int*>(static_cast<char*>(p) + bounds);      // bounds: a multiple of 16
+    sparse_min_tokens_ = min_tokens;
+    sparse_keep_ = n_keep;
+    sparse_sink_ = n_sink;
+    sparse_recent_ = n_recent;
+    // what is there already: the stream's own context and every open branch's.  Whatever stream wrote it has to be
+    // done, and the streams of the next steps find the bounds there.
+    drk_device_synchronize();
+    cm_->sync_block_table(stream);
+    paged_kv_bounds_update_batch(d_bounds_, pool.pool_ptr(), cm_->d_block_table(0), 0, ModelConfig::NUM_FA_LAYERS, 0, current_pos_, nb, bs,
+                                 stream);
+    for (size_t i = 0; i < branches_.size(); i++)
+        paged_kv_bounds_update_batch(d_bounds_, pool.pool_ptr(), cm_->d_block_table(branches_[i]), 0, ModelConfig::NUM_FA_LAYERS, 0,
+                                     pos_[i], nb, bs, stream);
+    if (drk_stream_synchronize(stream) != DRK_OK) LOG_ERROR("Conscientia", "KvStream: reading the context's bounds: %s", drk_last_error());
+    return true;
 }
 
 // Branches forked at different moments form a tree: all of them share the context up to the oldest fork, the
@@ -279,10 +341,7 @@ void KvStream::close_branches()
     positions_on_device_ = false;
     shared_tokens_ = 0;
     groups_.clear();
-    if (graph_) {                        // a captured step is tied to the branch set it was recorded for
-        drk_graph_destroy(graph_);
-        graph_ = nullptr;
-    }
+    drop_graph();                        // a captured step is tied to the branch set it was recorded for
 }
 
 bool KvStream::host_begin(hipStream_t stream)
@@ -345,7 +404,18 @@ void KvStream::decode_layer(int fa_layer_idx, const KvLayerIO& io, hipStream_t s
                                       d_pos_, B, fa_layer_idx, pool.max_blocks(), pool.block_size(), d_rope_table_,
                                       table_positions_, stream);
     const __half* gate = io.qg + hd;
-    if (scorer_ && scorer_->d_new_scores()) {
+    if (d_bounds_)
+        paged_kv_bounds_update_branches(d_bounds_, pool.pool_ptr(), tables, stride, d_pos_, B, fa_layer_idx, 1, pool.max_blocks(),
+                                        pool.block_size(), stream);
+    int min_len = pos_[0] + 1;
+    for (int p : pos_) min_len = p + 1 < min_len ? p + 1 : min_len;
+    if (d_bounds_ && min_len >= sparse_min_tokens_) {
+        paged_block_select_branches(ws_sparse_, d_bounds_, io.q_scratch, tables, stride, d_len_, B, max_len, sparse_keep_, sparse_sink_,
+                                    sparse_recent_, d_selected_, fa_layer_idx, pool.max_blocks(), pool.block_size(), stream);
+        paged_gqa_decode_attention_sparse(ws_sparse_, io.q_scratch, pool.pool_ptr(), tables, stride, d_len_, B, d_selected_,
+                                          sparse_keep_, gate, 2 * hd, io.attn_out, fa_layer_idx, pool.max_blocks(),
+                                          pool.block_size(), scale, stream);
+    } else if (scorer_ && scorer_->d_new_scores()) {
         if (first_layer_of_step_ < 0) first_layer_of_step_ = fa_layer_idx;
         float* mass = scorer_->d_new_scores() + (size_t)branches_[0] * stride;
         // the step's unit descriptors where the kernel takes a plan, the gate on the merge
@@ -409,10 +479,7 @@ void KvStream::end_decode_step(hipStream_t stream)
 bool KvStream::capture_decode_step(const std::function<void(hipStream_t)>& layers, hipStream_t stream)
 {
     if (branches_.empty()) return false;
-    if (graph_) {
-        drk_graph_destroy(graph_);
-        graph_ = nullptr;
-    }
+    drop_graph();
     // host part first: the capture must not contain table uploads or the position upload
     first_layer_of_step_ = -1;
     plan_built_ = false;

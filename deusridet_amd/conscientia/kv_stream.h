@@ -90,6 +90,17 @@ public:
     const std::vector<drk_prefix_group>& shared_groups() const { return groups_; }
     void set_shared_prefix_policy(int min_branches, int min_tokens) { shared_min_branches_ = min_branches; shared_min_tokens_ = min_tokens; }
 
+    // Decode over selected blocks (off by default): once every open branch is at least min_tokens long, a decode layer reads
+    // n_keep blocks per kv head -- the first n_sink, the last n_recent and the best others by the bounds of their
+    // keys -- instead of the whole context.  The bounds are kept from here on (perception and decode update them
+    // behind their writes; what the open branches and the stream hold already is read once, and waited for).  n_keep 0
+    // turns it off and frees the buffers.  False, and nothing changes, where the kernels do not take the geometry,
+    // with a scorer attached (it wants the attention mass of every block), with an overflow tier (a block that comes
+    // back may have lost its bounds), or when the device allocation fails.  Takes precedence over the shared-prefix
+    // paths.  Call it between steps; a captured step is dropped, and one captured afterwards keeps the path --
+    // selected or whole -- its branches' lengths called for when it was captured.
+    bool set_sparse_decode(int min_tokens, int n_keep, int n_sink, int n_recent, hipStream_t stream = nullptr);
+
     // One decode step = begin, decode_layer for every full-attention layer, end.
     // begin: blocks for the token each branch is about to write, table sync (this also issues the
     // copy-on-write copies), positions to the device when they are not there yet.
@@ -142,6 +153,14 @@ private:
     void* ev_attn_ = nullptr;              // a layer's attention call has been issued (recorded on the caller's stream)
     void* ev_mass_ = nullptr;              // its mass pass has been issued (recorded on the scorer's stream)
     bool mass_pending_ = false;
+
+    // decode over selected blocks: one allocation holds the bounds and the selection
+    void* d_bounds_ = nullptr;
+    int* d_selected_ = nullptr;            // [max_branches][kv heads][sparse_keep_]
+    AttentionWorkspace ws_sparse_;
+    int sparse_min_tokens_ = 0, sparse_keep_ = 0, sparse_sink_ = 0, sparse_recent_ = 0;
+    void drop_sparse();
+    void drop_graph();
 
     bool host_begin(hipStream_t stream);
     void host_end();

@@ -38,8 +38,11 @@ __device__ __forceinline__ void bounds_unpack(const uint4 &v, float scale, float
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             if constexpr (DT == DRK_INT8) {
+                // (code + 128) scale - 128 scale, rounded once: code * scale, exactly (a byte becomes a float in one
+                // instruction only if it is unsigned); a scale that is not finite gives NaN, which is passed over
+                const uint32_t u = w[i] ^ 0x80808080u;
 #pragma unroll
-                for (int j = 0; j < 4; j++) x[4 * i + j] = (float)(int8_t)(w[i] >> (8 * j)) * scale;
+                for (int j = 0; j < 4; j++) x[4 * i + j] = __fmaf_rn((float)(u >> (8 * j) & 0xffu), scale, -128.0f * scale);
             } else {
                 uint32_t lo, hi;
                 fp8x4_to_f16x4(w[i], lo, hi);
@@ -87,8 +90,8 @@ __device__ __forceinline__ void bounds_issue_barrier()
 #endif
 }
 
-// lowest and highest of 16 bytes of each of the rows r0, r0 + step, .. of a unit; 8 rows in flight
-template <int DT>
+// lowest and highest of 16 bytes of each of the rows r0, r0 + step, .. of a unit; B rows in flight
+template <int DT, int B>
 __device__ __forceinline__ void bounds_rows(const Lay &a, const BoundsArgs &A, const BoundsUnit &U, unsigned sub, int r0, int step,
                                             float *lo, float *hi)
 {
@@ -98,22 +101,23 @@ __device__ __forceinline__ void bounds_rows(const Lay &a, const BoundsArgs &A, c
     if (r0 >= U.cnt) return;
     const uint8_t *base = A.pool + row_off(a, U.layer, U.blk, 0, (int)U.h, 0) + sub * 16;
     const uint8_t *sc = A.pool + (DT == DRK_INT8 ? scale_off(a, U.layer, U.blk, 0, (int)U.h, 0) : 0);
-    for (int r = r0; r < U.cnt; r += 8 * step) {
-        uint4 v[8];
-        float s[8];
+    for (int r = r0; r < U.cnt; r += B * step) {
+        uint4 v[B];
+        float s[B];
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
+        for (int u = 0; u < B; u++) {
             const int rr = min(r + u * step, U.cnt - 1);               // a row read twice changes no bound
             v[u] = ld_stream128(base + (size_t)rr * a.row_bytes);
             s[u] = DT == DRK_INT8 ? f16_bits_to_f(*(const uint16_t *)(sc + (size_t)rr * 2)) : 1.0f;
         }
         bounds_issue_barrier();
 #pragma unroll
-        for (int u = 0; u < 8; u++) {
-            float x[V];
+        for (int u = 0; u < B; u += 2) {                               // two rows at a time: three-way minimum and maximum
+            float x[V], y[V];
             bounds_unpack<DT>(v[u], s[u], x);
+            bounds_unpack<DT>(v[u + 1], s[u + 1], y);
 #pragma unroll
-            for (int i = 0; i < V; i++) { lo[i] = fminf(lo[i], x[i]); hi[i] = fmaxf(hi[i], x[i]); }
+            for (int i = 0; i < V; i++) { lo[i] = fminf(fminf(lo[i], x[i]), y[i]); hi[i] = fmaxf(fmaxf(hi[i], x[i]), y[i]); }
         }
     }
 }
@@ -136,7 +140,7 @@ __global__ __launch_bounds__(kBThreads) void bounds_update_kernel(Lay a, BoundsA
     BoundsUnit U = {0, -1, 0, 0};
     if (unit < A.units) U = bounds_unit(a, A, (unsigned)unit);
     float lo[V], hi[V];
-    bounds_rows<DT>(a, A, U, sub, 0, 1, lo, hi);
+    bounds_rows<DT, 8>(a, A, U, sub, 0, 1, lo, hi);
     float amax = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; i++) {
@@ -181,7 +185,7 @@ __global__ __launch_bounds__(kBThreads) void bounds_update_long_kernel(Lay a, Bo
     const unsigned sub = threadIdx.x & (lpr - 1), rg = threadIdx.x >> lpr_shift;
     const int groups = (int)(kBThreads >> lpr_shift);
     float lo[V], hi[V];
-    bounds_rows<DT>(a, A, U, sub, (int)rg, groups, lo, hi);
+    bounds_rows<DT, 16>(a, A, U, sub, (int)rg, groups, lo, hi);
 #pragma unroll
     for (int i = 0; i < V; i += 4) {
         *(float4 *)&red[0][rg * a.D + sub * V + i] = make_float4(lo[i], lo[i + 1], lo[i + 2], lo[i + 3]);

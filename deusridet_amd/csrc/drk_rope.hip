@@ -92,9 +92,9 @@ __global__ __launch_bounds__(kRThreads) void rope_apply_kernel(RopeArgs A)
     const int u = (int)(it - row * A.units);
     const int t = (int)(row / A.row_groups), h0 = (int)(row - (size_t)t * A.row_groups);
     const bool rotated = u < A.hp;
-    // half-half: pair (i, i + r/2), so 8 pairs are chunks u and u + hp of 8; interleaved, or behind the rotary part: 16
-    // consecutive elements
-    const int e0 = A.interleaved || !rotated ? u * 16 : u * 8, e1 = A.interleaved || !rotated ? e0 + 8 : e0 + A.hp * 8;
+    // chunks u and u + hp of 8 elements: half-half, pair (i, i + r/2), they are 8 pairs; interleaved 4 pairs each.  Behind the
+    // rotary part likewise.  Neighbouring lanes are on neighbouring chunks in both accesses.
+    const int e0 = rotated ? u * 8 : A.hp * 16 + (u - A.hp) * 8, e1 = e0 + (rotated ? A.hp : A.units - A.hp) * 8;
     uint4 va[HPT], vb[HPT];
     uint16_t *o[HPT];
 #pragma unroll
@@ -114,7 +114,7 @@ __global__ __launch_bounds__(kRThreads) void rope_apply_kernel(RopeArgs A)
         const double p = A.d_pos ? A.d_pos[t] : (double)A.pos_start + t;
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            rope_cos_sin(p, A.freqs[u * 8 + i], c[i], s[i]);
+            rope_cos_sin(p, A.freqs[A.interleaved ? (i < 4 ? u : u + A.hp - 1) * 4 + i : u * 8 + i], c[i], s[i]);
             c[i] *= A.cm;
             s[i] *= A.sm;
         }

@@ -26,7 +26,7 @@ namespace drk {
 
 constexpr uint32_t kKeyForced = 0xffffffffu;
 constexpr int kSelFused = 1024;         // blocks of a context up to which one workgroup scores and selects
-constexpr size_t kSelWaves = 8192, kSelTileWgs = 512;     // waves / workgroups the scores are spread over
+constexpr size_t kSelWaves = 8192, kSelTileWgs = 256;     // waves / workgroups the scores are spread over
 typedef int sel_i32x4 __attribute__((ext_vector_type(4)));
 
 struct SelArgs {

@@ -444,12 +444,16 @@ static int sparse_pieces(const Lay &a, int T, int n_keep, int *groups_per_piece)
     return (int)((groups + *groups_per_piece - 1) / *groups_per_piece);
 }
 
-// Waves per row: as few as still give the chip the waves it holds (16 per CU at head_dim 128, 8 at 256).
-static int sparse_waves_per_row(const Lay &a, int T)
+// Waves per row: as few as still give the chip the waves it holds (16 per CU at head_dim 128, 8 at 256) and leave
+// room in LDS for that many.
+static int sparse_waves_per_row(const Lay &a, int T, int groups_per_piece)
 {
     const size_t rows = (size_t)T * a.KVH, waves = a.D == 128 ? 4096 : 2048;
+    const unsigned pitch = (unsigned)a.D * 2 + 16, staged = kSpWaves * 16 * pitch + 2048, room = (a.D == 128 ? 80u : 160u) << 10;
     int w = 8;
-    while (w > 1 && rows * (w / 2) >= waves) w /= 2;
+    while (w > 1 && rows * (w / 2) >= waves &&
+           staged + sparse_lds(a.QH / a.KVH, (int)pitch, groups_per_piece, a.dtype == DRK_INT8, kSpWaves / (w / 2)).total <= room)
+        w /= 2;
     return w;
 }
 
@@ -527,7 +531,7 @@ int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void
     A.scale_log2e = scale * kSLog2e;
     hipStream_t st = (hipStream_t)stream;
     const bool shared = table_stride == 0 && T > 1;           // rows over one table meet in the same pages: keep them cached
-    const int wpr = A.pieces > 1 ? 8 : sparse_waves_per_row(a, T);
+    const int wpr = A.pieces > 1 ? 8 : sparse_waves_per_row(a, T, A.groups_per_piece);
     const dim3 grid((unsigned)(((size_t)T * wpr + 7) / 8 * A.pieces * a.KVH));
 #define DRK_SPARSE_LAUNCH4(DT, D, NT, WPR)                                                                                  \
     hipLaunchKernelGGL((sparse_kernel<DT, D, NT, WPR>), grid, dim3(kSpWaves * 64),                                          \

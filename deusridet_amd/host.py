@@ -100,6 +100,7 @@ SIGNATURES = {
     "drkh_kvs_branch_pos": (_i32, [_vp, _i32]),
     "drkh_kvs_shared_tokens": (_i32, [_vp]),
     "drkh_kvs_set_shared_prefix_policy": (None, [_vp, _i32, _i32]),
+    "drkh_kvs_set_sparse_decode": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp]),
     "drkh_kvs_begin_decode_step": (_i32, [_vp, _vp]),
     "drkh_kvs_decode_layer": (None, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "drkh_kvs_end_decode_step": (None, [_vp, _vp]),
@@ -208,6 +209,8 @@ class KvStream:
     def set_branch_count(self, n): return lib().drkh_kvs_set_branch_count(self._h, n)
     def shared_tokens(self): return lib().drkh_kvs_shared_tokens(self._h)
     def set_shared_prefix_policy(self, min_branches, min_tokens): lib().drkh_kvs_set_shared_prefix_policy(self._h, min_branches, min_tokens)
+    def set_sparse_decode(self, min_tokens, n_keep, n_sink, n_recent, stream=None):
+        return bool(lib().drkh_kvs_set_sparse_decode(self._h, min_tokens, n_keep, n_sink, n_recent, stream))
     def close_branches(self): lib().drkh_kvs_close_branches(self._h)
     def num_branches(self): return lib().drkh_kvs_num_branches(self._h)
     def branch_id(self, i): return lib().drkh_kvs_branch_id(self._h, i)

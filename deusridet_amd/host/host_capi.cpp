@@ -310,6 +310,10 @@ int drkh_kvs_branch_id(void *ks, int i) { return KS(ks)->branch_id(i); }
 int drkh_kvs_branch_pos(void *ks, int i) { return KS(ks)->branch_pos(i); }
 int drkh_kvs_shared_tokens(void *ks) { return KS(ks)->shared_tokens(); }
 void drkh_kvs_set_shared_prefix_policy(void *ks, int min_branches, int min_tokens) { KS(ks)->set_shared_prefix_policy(min_branches, min_tokens); }
+int drkh_kvs_set_sparse_decode(void *ks, int min_tokens, int n_keep, int n_sink, int n_recent, void *stream)
+{
+    return KS(ks)->set_sparse_decode(min_tokens, n_keep, n_sink, n_recent, ST(stream)) ? 1 : 0;
+}
 int drkh_kvs_begin_decode_step(void *ks, void *stream) { return KS(ks)->begin_decode_step((hipStream_t)stream) ? 1 : 0; }
 void drkh_kvs_decode_layer(void *ks, int fa_layer_idx, const void *qg, const void *k, const void *v, const void *q_norm,
                            const void *k_norm, void *q_scratch, void *attn_out, void *stream)

@@ -20,6 +20,12 @@ void sigmoid_gate(const __half* x, const __half* gate, __half* out, int n, hipSt
 void apply_rope(__half* q, __half* k, int num_heads, int num_kv_heads, int head_dim, int rotary_dim, const int* d_pos,
                 float theta, hipStream_t stream = 0);
 
+// Rotary positions for contexts beyond the trained one (not in the reference): frequencies stretched as `rope` says,
+// half-half or interleaved pairs, T tokens of q [T, num_heads, head_dim] and k [T, num_kv_heads, head_dim] in place, at
+// d_pos[t] or, with a null d_pos, at pos_start + t.  d_freqs: see drk_rope_freqs_fill.  inverse: the gradient.
+void apply_rope_scaled(const drk_rope& rope, const double* d_freqs, __half* q, __half* k, int T, int num_heads, int num_kv_heads,
+                       int head_dim, const int* d_pos, int pos_start, bool inverse = false, hipStream_t stream = 0);
+
 // Per-head RMSNorm: x, out [num_heads, head_dim], weight [head_dim]
 void head_norm(const __half* x, const __half* weight, __half* out, int num_heads, int head_dim, float eps,
                hipStream_t stream = 0);

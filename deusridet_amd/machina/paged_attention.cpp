@@ -69,6 +69,15 @@ void AttentionWorkspace::release()
     bytes_ = 0;
 }
 
+void AttentionWorkspace::adopt(AttentionWorkspace& other)
+{
+    if (ptr_ || this == &other) return;
+    ptr_ = other.ptr_;
+    bytes_ = other.bytes_;
+    other.ptr_ = nullptr;
+    other.bytes_ = 0;
+}
+
 // ---- one workspace per stream for the calls that take none ---------------------------------
 
 namespace {
@@ -202,6 +211,106 @@ void paged_gqa_decode_attention_shared(AttentionWorkspace& ws, const __half* Q, 
                                           shared_tokens, out, fa_layer_idx, scale, ModelConfig::IO_DTYPE, ws.ptr(),
                                           ws.bytes(), stream) != DRK_OK)
         LOG_ERROR("Machina", "paged_gqa_decode_attention_shared: %s", drk_last_error());
+}
+
+// ---- attention over selected blocks ---------------------------------------------------------
+
+bool paged_sparse_attention_supported(int block_size)
+{
+    return (ModelConfig::HEAD_DIM == 128 || ModelConfig::HEAD_DIM == 256) && block_size > 0 && block_size % 16 == 0 &&
+           ModelConfig::NUM_KV_HEADS > 0 && ModelConfig::NUM_ATTN_HEADS / ModelConfig::NUM_KV_HEADS <= 16;
+}
+
+size_t paged_kv_bounds_bytes(int max_phys_blocks, int block_size)
+{
+    drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
+    return drk_kv_bounds_bytes(&g);
+}
+
+size_t paged_sparse_workspace_bytes(int max_rows, int max_seq_len, int n_keep, int max_phys_blocks, int block_size)
+{
+    // The selection's need grows with the rows; the attention's does not have to (the more rows, the fewer pieces): take
+    // the largest of every number of rows up to the most that are ever cut.
+    drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
+    size_t need = drk_block_select_workspace_bytes(&g, max_rows, max_seq_len);
+    for (int rows = 1; rows <= max_rows && rows <= 512; rows++) {
+        const size_t n = drk_paged_sparse_workspace_bytes(&g, rows, n_keep);
+        need = n > need ? n : need;
+    }
+    const size_t n = drk_paged_sparse_workspace_bytes(&g, max_rows, n_keep);
+    return n > need ? n : need;
+}
+
+void paged_kv_bounds_update_batch(void* d_bounds, const __half* kv_pool, const int* d_block_table, int fa_layer_idx,
+                                  int num_layers, int pos_start, int M, int max_phys_blocks, int block_size, hipStream_t stream)
+{
+    if (M <= 0) return;
+    drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
+    if (drk_kv_bounds_update(&g, kv_pool, d_block_table, 0, nullptr, pos_start, M, fa_layer_idx, num_layers, d_bounds, stream) != DRK_OK)
+        LOG_ERROR("Machina", "paged_kv_bounds_update_batch: %s", drk_last_error());
+}
+
+void paged_kv_bounds_update_branches(void* d_bounds, const __half* kv_pool, const int* d_tables, int table_stride,
+                                     const int* d_pos, int B, int fa_layer_idx, int num_layers, int max_phys_blocks,
+                                     int block_size, hipStream_t stream)
+{
+    if (B <= 0) return;
+    drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
+    if (!d_pos)
+        LOG_ERROR("Machina", "paged_kv_bounds_update_branches: d_pos is null");
+    else if (drk_kv_bounds_update(&g, kv_pool, d_tables, table_stride, d_pos, 0, B, fa_layer_idx, num_layers, d_bounds, stream) != DRK_OK)
+        LOG_ERROR("Machina", "paged_kv_bounds_update_branches: %s", drk_last_error());
+}
+
+void paged_block_select_branches(AttentionWorkspace& ws, const void* d_bounds, const __half* Q, const int* d_tables,
+                                 int table_stride, const int* d_seq_lens, int B, int max_seq_len, int n_keep, int n_sink,
+                                 int n_recent, int* d_selected, int fa_layer_idx, int max_phys_blocks, int block_size,
+                                 hipStream_t stream)
+{
+    if (B <= 0) return;
+    drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
+    if (!d_seq_lens)
+        LOG_ERROR("Machina", "paged_block_select_branches: d_seq_lens is null");
+    else if (drk_block_select(&g, d_bounds, fa_layer_idx, Q, ModelConfig::IO_DTYPE, d_tables, table_stride, d_seq_lens, 0, B,
+                              max_seq_len, n_keep, n_sink, n_recent, d_selected, ws.ptr(), ws.bytes(), stream) != DRK_OK)
+        LOG_ERROR("Machina", "paged_block_select_branches: %s", drk_last_error());
+}
+
+void paged_block_select_prefill(AttentionWorkspace& ws, const void* d_bounds, const __half* Q, const int* d_block_table,
+                                int pos_start, int M, int n_keep, int n_sink, int n_recent, int* d_selected,
+                                int fa_layer_idx, int max_phys_blocks, int block_size, hipStream_t stream)
+{
+    if (M <= 0) return;
+    drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
+    if (drk_block_select(&g, d_bounds, fa_layer_idx, Q, ModelConfig::IO_DTYPE, d_block_table, 0, nullptr, pos_start, M, pos_start + M,
+                         n_keep, n_sink, n_recent, d_selected, ws.ptr(), ws.bytes(), stream) != DRK_OK)
+        LOG_ERROR("Machina", "paged_block_select_prefill: %s", drk_last_error());
+}
+
+void paged_gqa_decode_attention_sparse(AttentionWorkspace& ws, const __half* Q, const __half* kv_pool, const int* d_tables,
+                                       int table_stride, const int* d_seq_lens, int B, const int* d_selected, int n_keep,
+                                       const __half* gate, int gate_stride, __half* out, int fa_layer_idx, int max_phys_blocks,
+                                       int block_size, float scale, hipStream_t stream)
+{
+    if (B <= 0) return;
+    drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
+    if (!d_seq_lens)
+        LOG_ERROR("Machina", "paged_gqa_decode_attention_sparse: d_seq_lens is null");
+    else if (drk_paged_sparse_attention(&g, Q, kv_pool, d_tables, table_stride, d_seq_lens, 0, B, d_selected, n_keep, out, fa_layer_idx,
+                                        scale, ModelConfig::IO_DTYPE, gate, (size_t)gate_stride, ws.ptr(), ws.bytes(), stream) != DRK_OK)
+        LOG_ERROR("Machina", "paged_gqa_decode_attention_sparse: %s", drk_last_error());
+}
+
+void paged_prefill_attention_sparse(AttentionWorkspace& ws, const __half* Q, const __half* kv_pool, const int* d_block_table,
+                                    const int* d_selected, int n_keep, const __half* gate, int gate_stride, __half* out,
+                                    int fa_layer_idx, int pos_start, int M, int max_phys_blocks, int block_size, float scale,
+                                    hipStream_t stream)
+{
+    if (M <= 0) return;
+    drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
+    if (drk_paged_sparse_attention(&g, Q, kv_pool, d_block_table, 0, nullptr, pos_start, M, d_selected, n_keep, out, fa_layer_idx, scale,
+                                   ModelConfig::IO_DTYPE, gate, (size_t)gate_stride, ws.ptr(), ws.bytes(), stream) != DRK_OK)
+        LOG_ERROR("Machina", "paged_prefill_attention_sparse: %s", drk_last_error());
 }
 
 size_t paged_decode_plan_bytes(int B, int max_seq_len, int max_phys_blocks, int block_size, int n_groups)

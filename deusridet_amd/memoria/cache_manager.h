@@ -101,6 +101,8 @@ public:
     void release_branch(int branch);
     bool branch_alive(int branch) const;
     int  max_branches() const { return max_branches_; }
+    // Evicted blocks go to an overflow tier and may come back in other physical blocks (an initialised swapper).
+    bool has_overflow_tier() const { return ssd_enabled_; }
     // Tokens [0, n) whose pages are the same physical blocks in every listed branch
     // (whole blocks only, capped by the shortest seq_len): what
     // paged_gqa_decode_attention_shared() may stream once for all of them.

@@ -517,7 +517,8 @@ int drk_rope_apply(const drk_rope *r, const double *d_freqs, const drk_rope_rows
  * as int8 codes of one power of two, rounded outward:
  *   e = the smallest whole number in [-40, 40] with max |k| <= 127 * 2^e  (40 if there is none: values beyond are
  *   taken as +-127 * 2^40),  low = floor(min k / 2^e),  high = ceil(max k / 2^e).
- * NaN keys are passed over (a dimension that holds nothing else has low = high = 0).
+ * NaN keys, and int8 tokens whose scale is not finite, are passed over (a dimension that holds nothing else has
+ * low = high = 0).
  * Buffer of drk_kv_bounds_bytes(): codes int8 [layers][blocks][kv heads][2 (low, high)][head_dim], then exponents
  * int8 [layers][blocks][kv heads]; 16-byte aligned.  It need not be cleared: entries mean something once updated.
  * head_dim is a power of two in [64, 512], any storage type, any block size. */

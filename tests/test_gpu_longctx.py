@@ -243,6 +243,25 @@ def test_bounds_of_extreme_keys(dev, dtype):
         check_block(p, codes, exps, 0, blk, 4)
 
 
+def test_bounds_of_int8_tokens_without_a_finite_scale(dev):
+    rng = np.random.default_rng(11)
+    p = R.Pool(rng, 1, 2, 2, 128, 16, 3, cabi.INT8)
+    sc = p.raw[0][:, 2 * 2 * 16 * 128:].view(np.uint16).reshape(3, 2, 2, 16)
+    sc[1, 0, 0, [2, 5, 7]] = [0x7FFF, 0x7C00, 0xFC00]                   # NaN, infinities
+    sc[2, 0, 1] = 0x7E00                                                # nothing else
+    sc[1, 0, 1, 4] = 0x7BFF                                             # the largest finite one
+    p.k = p.raw[0][:, :2 * 2 * 16 * 128].view(np.int8).reshape(3, 2, 2, 16, 128)[:, 0].astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        s = sc[:, 0].view(np.float16).astype(np.float64)
+        p.k = (p.k * np.where(np.isfinite(s), s, np.nan)[..., None])[None]
+    db, dp, dt = bounds_dev(p), U.dev_bytes(p.raw), U.dev_i32(np.arange(3))
+    cabi.call("drk_kv_bounds_update", p.g, U.p(dp), U.p(dt), 0, None, 0, 48, 0, 1, U.p(db), U.stream_ptr())
+    U.sync()
+    codes, exps = bounds_host(p, db)
+    for blk in range(3):
+        check_block(p, codes, exps, 0, blk, 16)
+
+
 # ---- selection --------------------------------------------------------------------------------
 def run_select(g, raw, q, tables, stride, lens, start, T, max_len, keep, sink, recent, io, layer=0, shift=0):
     dsel = U.dev_i32(np.full(T * g.num_kv_heads * keep + 4, 77, np.int32))
@@ -295,6 +314,26 @@ def test_select_chunk(dev, D, QH, KVH, T, start):
     qf = U.from_bits(q, io).astype(np.float64)
     for t in range(T):
         assert np.array_equal(got[t], R.select(qf[t], codes[0], exps[0], table, start + t + 1, bs, keep, sink, recent)), t
+
+
+@pytest.mark.parametrize("D,QH,KVH,T", [(128, 8, 2, 70), (256, 6, 1, 37), (64, 2, 2, 21), (128, 16, 1, 9), (512, 3, 3, 11)])
+def test_select_rows_of_any_length_over_one_table(dev, D, QH, KVH, T):
+    """One table, a length per row (none, one, ragged, beyond max_seq_len); more blocks than one workgroup selects from."""
+    rng = np.random.default_rng(D * T)
+    bs, n, keep, sink, recent, io = 4, 1400, 19, 1, 3, cabi.F16
+    table = U.shuffled_table(rng, n, n)
+    table[rng.random(n) < 0.05] = -1
+    lens = rng.integers(-1, n * bs + 1, T).astype(np.int32)
+    lens[:6] = [0, 1, n * bs, 5000, 4097, 4096]
+    g = cabi.layout(1, KVH, QH, D, bs, n, cabi.INT8)
+    codes, exps = R.bounds_buffers(1, n, KVH, D, rng)
+    q = U.normal_bits(rng, (T, QH, D), io)
+    qf = U.from_bits(q, io).astype(np.float64)
+    for most in (n * bs, 4500):
+        got = run_select(g, R.bounds_bytes(codes, exps), q, table, 0, lens, 0, T, most, keep, sink, recent, io)
+        for t in range(T):
+            want = R.select(qf[t], codes[0], exps[0], table, min(int(lens[t]), most), bs, keep, sink, recent)
+            assert np.array_equal(got[t], want), (most, t)
 
 
 @pytest.mark.parametrize("kind", ["equal", "few", "extreme"])
@@ -358,9 +397,9 @@ def run_attend(p, q, tables, stride, lens, start, sel, io, layer=0, gate=None, g
     return U.host(do, np.uint16, out.shape)
 
 
-def check_attend(p, got, q, tables, lens, sel, io, layer=0, gate=None, scale=None):
+def check_attend(p, got, q, tables, lens, sel, io, layer=0, gate=None, scale=None, rows=None):
     worst = 0.0
-    for t in range(q.shape[0]):
+    for t in range(q.shape[0]) if rows is None else rows:
         tab = tables[t] if tables.ndim == 2 else tables
         want, tol = R.attend(p, layer, U.from_bits(q[t], io).astype(np.float64), tab, int(lens[t]), sel[t], scale or 1 / math.sqrt(p.D),
                              None if gate is None else U.from_bits(gate[t], io).astype(np.float64))
@@ -444,6 +483,43 @@ def test_attend_chunk(dev, dtype, T, keep):
     q = U.normal_bits(rng, (T, QH, D), io, 1.5)
     got = run_attend(p, q, table, 0, None, start, sel, io)
     check_attend(p, got, q, table, start + 1 + np.arange(T), sel, io)
+
+
+@pytest.mark.parametrize("dtype", [cabi.BF16, cabi.INT8])
+@pytest.mark.parametrize("D,T", [(128, 130), (128, 261), (128, 515), (256, 131), (256, 300)])
+@pytest.mark.parametrize("mode", ["chunk", "branches"])
+def test_attend_many_rows(dev, dtype, D, T, mode):
+    """Row counts from which a workgroup takes two, four or eight rows instead of one; the last workgroup is not full."""
+    rng = np.random.default_rng(T)
+    QH, KVH, bs, n, keep, start = 16, 8, 16, 12, 5, 40
+    io = dtype if dtype < cabi.INT8 else cabi.F16
+    chunk = mode == "chunk"
+    n = -(-(start + T) // bs) if chunk else n
+    NB = n + 3 if chunk else 40
+    p = R.Pool(rng, 1, KVH, QH, D, bs, NB, dtype)
+    tables = U.shuffled_table(rng, NB, n) if chunk else rng.integers(0, NB, (T, n)).astype(np.int32)
+    lens = start + 1 + np.arange(T) if chunk else rng.integers(0, n * bs + 1, T)
+    sel = np.sort(rng.integers(-1, n, (T, KVH, keep)).astype(np.int32), axis=2)
+    sel[3], sel[T - 1, 2:] = -1, -1
+    q = U.normal_bits(rng, (T, QH, D), io)
+    gate = U.normal_bits(rng, (T, QH, D), io)
+    got = run_attend(p, q, tables, 0 if chunk else n, None if chunk else lens.astype(np.int32), start if chunk else 0, sel, io, 0, gate, D)
+    check_attend(p, got, q, tables, lens, sel, io, 0, gate)
+
+
+@pytest.mark.parametrize("D,KVH,T,dtype", [(256, 1, 2100, cabi.INT8), (128, 1, 4100, cabi.INT8), (128, 2, 4096, cabi.BF16)])
+def test_attend_many_rows_of_long_lists(dev, D, KVH, T, dtype):
+    """16 query heads per kv head and 512 groups per row: what a workgroup keeps in LDS limits the rows it takes."""
+    rng = np.random.default_rng(D + T)
+    bs, n, keep, G = 256, 40, 32, 16
+    io = dtype if dtype < cabi.INT8 else cabi.BF16
+    p = R.Pool(rng, 1, KVH, KVH * G, D, bs, n, dtype)
+    table = rng.permutation(n).astype(np.int32)
+    sel = np.argsort(rng.random((T, KVH, n)), axis=2)[..., :keep].astype(np.int32)
+    start = n * bs - T - 5
+    q = U.normal_bits(rng, (T, KVH * G, D), io)
+    got = run_attend(p, q, table, 0, None, start, sel, io)
+    check_attend(p, got, q, table, start + 1 + np.arange(T), sel, io, rows=[0, 1, 7, 8, T // 2 + 1, T - 9, T - 1])
 
 
 def test_attend_everything_equals_dense_decode(dev):

@@ -240,6 +240,25 @@ void drkh_apply_rope(void *q, void *k, int num_heads, int num_kv_heads, int head
 {
     apply_rope(H(q), H(k), num_heads, num_kv_heads, head_dim, rotary_dim, d_pos, theta, (hipStream_t)stream);
 }
+void drkh_apply_rope_scaled(const drk_rope *rope, const double *d_freqs, void *q, void *k, int T, int num_heads, int num_kv_heads,
+                            int head_dim, const int32_t *d_pos, int pos_start, int inverse, void *stream)
+{
+    apply_rope_scaled(*rope, d_freqs, H(q), H(k), T, num_heads, num_kv_heads, head_dim, d_pos, pos_start, inverse != 0, ST(stream));
+}
+int drkh_paged_prefill_sparse(const void *Q, const void *pool, void *d_bounds, const int32_t *d_block_table, int pos_start, int M,
+                              int n_keep, int n_sink, int n_recent, int32_t *d_selected, const void *gate, int gate_stride,
+                              void *out, int fa_layer_idx, int max_phys_blocks, int block_size, float scale, void *stream)
+{
+    AttentionWorkspace ws;
+    const size_t need = paged_sparse_workspace_bytes(M, pos_start + M, n_keep, max_phys_blocks, block_size);
+    if (need == 0 || !ws.reserve(need)) return 0;
+    paged_kv_bounds_update_batch(d_bounds, CH(pool), d_block_table, fa_layer_idx, 1, 0, pos_start + M, max_phys_blocks, block_size, ST(stream));
+    paged_block_select_prefill(ws, d_bounds, CH(Q), d_block_table, pos_start, M, n_keep, n_sink, n_recent, d_selected, fa_layer_idx,
+                               max_phys_blocks, block_size, ST(stream));
+    paged_prefill_attention_sparse(ws, CH(Q), CH(pool), d_block_table, d_selected, n_keep, CH(gate), gate_stride, H(out), fa_layer_idx,
+                                   pos_start, M, max_phys_blocks, block_size, scale, ST(stream));
+    return drk_stream_synchronize(stream) == DRK_OK ? 1 : 0;
+}
 void drkh_head_norm(const void *x, const void *weight, void *out, int num_heads, int head_dim, float eps,
                     void *stream)
 {

@@ -156,6 +156,14 @@ void drkh_paged_gqa_decode_attention_gated_branches(const void *Q, void *kv_pool
 void drkh_paged_prefill_attention_gated(const void *Q, void *kv_pool, const int32_t *d_block_table, const void *gate,
                                         int gate_stride, void *out, int fa_layer_idx, int pos_start, int M,
                                         int max_phys_blocks, int block_size, float scale, void *stream);
+struct drk_rope;                 /* drk_kv.h */
+/* apply_rope_scaled (layer.h); a chunk of M tokens over selected blocks: paged_kv_bounds_update_batch, paged_block_select_prefill
+ * and paged_prefill_attention_sparse (paged_attention.h) on a workspace of its own, waited for; 0 when that cannot be had */
+void drkh_apply_rope_scaled(const struct drk_rope *rope, const double *d_freqs, void *q, void *k, int T, int num_heads, int num_kv_heads,
+                            int head_dim, const int32_t *d_pos, int pos_start, int inverse, void *stream);
+int  drkh_paged_prefill_sparse(const void *Q, const void *pool, void *d_bounds, const int32_t *d_block_table, int pos_start, int M,
+                               int n_keep, int n_sink, int n_recent, int32_t *d_selected, const void *gate, int gate_stride,
+                               void *out, int fa_layer_idx, int max_phys_blocks, int block_size, float scale, void *stream);
 /* conscientia/kv_stream.h: the KV side of ConscientiStream (src/conscientia/stream.cpp:145-401) */
 void *drkh_kvs_create(void);
 void  drkh_kvs_destroy(void *ks);

@@ -6,7 +6,7 @@ import math
 import numpy as np
 import pytest
 
-from deusridet_amd import cabi
+from deusridet_amd import cabi, host
 from tests import longctx_ref as R
 from tests import util as U
 
@@ -109,6 +109,54 @@ def test_rope_apply_in_place_three_tensors_and_head_major(dev, interleaved):
     want, mag = R.rope(r, U.from_bits(q, dtype).transpose(1, 0, 2), 777 + np.arange(T))
     got = U.from_bits(U.host(oq, np.uint16, q.shape), dtype).astype(np.float64).transpose(1, 0, 2)
     rope_ok(got, None, want, mag, dtype, np.arange(D) < 64)
+
+
+@pytest.mark.parametrize("dtype", [cabi.F16, cabi.BF16])
+def test_scaled_table_in_the_fused_layer_step(dev, dtype):
+    """The fused norm + rotation + append reads a table of stretched angles: its keys in the pages and its queries equal the
+    norm followed by the rotation that forms the angles itself, but for the two roundings in between."""
+    import torch
+    rng = np.random.default_rng(8)
+    D, QH, KVH, bs, T, start = 128, 4, 2, 16, 21, 4000
+    r = cabi.rope(64, False, 1e6, 8.0, 1024.0, 1.0, 32.0, 1.2)
+    g = cabi.layout(1, KVH, QH, D, bs, 300, dtype)
+    pool = U.dev_zeros(cabi.lib().drk_kv_pool_bytes(C.byref(g)))
+    table = U.dev_i32(np.arange(300))
+    npos = start + T
+    tab = torch.zeros(npos * 64, dtype=torch.float32, device="cuda")
+    cabi.call("drk_rope_table_fill_scaled", r, U.p(tab), npos, U.stream_ptr())
+    qg, k, v, w = (U.normal_bits(rng, s, dtype) for s in ((T, QH, 2 * D), (T, KVH, D), (T, KVH, D), (D,)))
+    dqg, dk, dv, dw, dq = U.dev_bytes(qg), U.dev_bytes(k), U.dev_bytes(v), U.dev_bytes(w), U.dev_zeros(T * QH * D * 2)
+    cabi.call("drk_qk_norm_rope_append", g, U.p(pool), U.p(table), 300, None, start, T, 0, U.p(dqg), U.p(dk), U.p(dv), U.p(dw), U.p(dw), 1e-6, 64,
+              r.theta, U.p(tab), npos, U.p(dq), dtype, U.stream_ptr())
+    U.sync()
+    pages = U.from_bits(U.host(pool, np.uint16, (300, 2, KVH, bs, D)), dtype).astype(np.float64)
+    got_k = np.stack([pages[p // bs, 0, :, p % bs] for p in range(start, npos)])
+    got_q = U.from_bits(U.host(dq, np.uint16, (T, QH, D)), dtype).astype(np.float64)
+    for got, x in ((got_q, qg[..., :D]), (got_k, k)):
+        xf, wf = U.from_bits(x, dtype).astype(np.float64), U.from_bits(w, dtype).astype(np.float64)
+        n = xf / np.sqrt((xf ** 2).mean(-1, keepdims=True) + 1e-6) * wf
+        want, mag = R.rope(r, n, start + np.arange(T))
+        mag[..., 64:] = np.abs(n[..., 64:])
+        h = R.HALF_STEP[dtype]
+        lim = h * 1.01 * mag + h * (np.abs(want) + 2 * h * mag) + 2.0 ** -20 * mag + (2.0 ** -23 if dtype == cabi.F16 else 0)
+        assert (np.abs(got - want) <= lim).all()
+
+
+def test_rope_through_the_host_class_in_place(dev):
+    rng = np.random.default_rng(31)
+    T, D, dtype = 5, 128, cabi.BF16
+    assert host.set_attention_geometry(1, 8, 2, D, dtype, dtype)
+    r = cabi.rope(96, True, 1e4, 16.0, 4096.0, 1.0, 32.0, 1.1)
+    f = freqs_of(r)
+    q, k = U.normal_bits(rng, (T, 8, D), dtype), U.normal_bits(rng, (T, 2, D), dtype)
+    dq, dk = U.dev_bytes(q), U.dev_bytes(k)
+    host.lib().drkh_apply_rope_scaled(r, U.p(f), U.p(dq), U.p(dk), T, 8, 2, D, None, 70000, 1, U.stream_ptr())
+    U.sync()
+    for buf, x in ((dq, q), (dk, k)):
+        xf = U.from_bits(x, dtype).astype(np.float64)
+        want, mag = R.rope(r, xf, 70000 + np.arange(T), True)
+        rope_ok(U.from_bits(U.host(buf, np.uint16, x.shape), dtype).astype(np.float64), xf, want, mag, dtype, np.arange(D) < 96)
 
 
 def test_rope_inverse_is_the_gradient(dev):
@@ -565,6 +613,33 @@ def test_attend_nan_and_infinities_in_listed_tokens(dev):
     _, tol = R.attend(p, 0, U.from_bits(q[1], cabi.F16).astype(np.float64), tables[1], n * bs, less, 1 / math.sqrt(D))
     ok, r = R.attend_ok(U.from_bits(got[1], cabi.F16), want, 2 * tol, cabi.F16)
     assert ok, r
+
+
+@pytest.mark.parametrize("dtype", [cabi.BF16, cabi.FP8_E4M3])
+def test_chunk_over_selected_blocks_through_the_host_functions(dev, dtype):
+    """Bounds of the context, selection and attention of a chunk's rows, as a model's prefill would call them."""
+    rng = np.random.default_rng(40)
+    D, QH, KVH, bs, start, M, keep, sink, recent = 128, 8, 2, 16, 411, 45, 7, 1, 2
+    io = cabi.BF16
+    assert host.set_attention_geometry(2, QH, KVH, D, dtype, io)
+    n = -(-(start + M) // bs)
+    p = R.Pool(rng, 2, KVH, QH, D, bs, n + 4, dtype, 1.5)
+    table = U.shuffled_table(rng, n + 4, n)
+    table[9] = -1
+    q, gate = U.normal_bits(rng, (M, QH, D), io), U.normal_bits(rng, (M, QH, D), io)
+    dq, dp, dt, dg, db = U.dev_bytes(q), U.dev_bytes(p.raw), U.dev_i32(table), U.dev_bytes(gate), bounds_dev(p)
+    dsel, do = U.dev_i32(np.zeros((M, KVH, keep))), U.dev_zeros(q.nbytes)
+    assert host.lib().drkh_paged_prefill_sparse(U.p(dq), U.p(dp), U.p(db), U.p(dt), start, M, keep, sink, recent, U.p(dsel), U.p(dg), D, U.p(do),
+                                                1, n + 4, bs, 1 / math.sqrt(D), U.stream_ptr())
+    codes, exps = bounds_host(p, db)
+    sel = U.host(dsel, np.int32, (M, KVH, keep))
+    qf = U.from_bits(q, io).astype(np.float64)
+    for lb in range(n):
+        if table[lb] >= 0:
+            check_block(p, codes, exps, 1, table[lb], min(bs, start + M - lb * bs))
+    for t in range(M):
+        assert np.array_equal(sel[t], R.select(qf[t], codes[1], exps[1], table, start + t + 1, bs, keep, sink, recent)), t
+    check_attend(p, U.host(do, np.uint16, q.shape), q, table, start + 1 + np.arange(M), sel, io, 1, gate)
 
 
 # ---- together ---------------------------------------------------------------------------------

@@ -5,6 +5,7 @@ raises ImportError: nothing here computes anything on its own.
 """
 import ctypes as C
 import os
+import struct
 import sys
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -68,7 +69,10 @@ class RopeRows(C.Structure):
 def rope_rows(tensors):
     """ctypes array of drk_rope_rows from (x, out, heads, x token stride, x head stride, out token stride, out head
     stride) tuples: addresses, and strides in elements"""
-    return (RopeRows * len(tensors))(*[(x, out, heads, 0, *strides) for x, out, heads, *strides in tensors])
+    flat = []
+    for x, out, heads, *strides in tensors:
+        flat += (x or 0, out or 0, heads, 0, *strides)
+    return (RopeRows * len(tensors)).from_buffer_copy(struct.pack("PPii4N" * len(tensors), *flat))
 
 
 _vp, _i32, _sz, _f32 = C.c_void_p, C.c_int32, C.c_size_t, C.c_float

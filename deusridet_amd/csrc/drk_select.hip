@@ -25,8 +25,14 @@
 namespace drk {
 
 constexpr uint32_t kKeyForced = 0xffffffffu;
-constexpr int kSelFused = 1024;         // blocks of a context up to which one workgroup scores and selects
-constexpr size_t kSelWaves = 8192, kSelTileWgs = 256;     // waves / workgroups the scores are spread over
+// Contexts of few blocks are scored and selected by one workgroup per (row, kv head) in one launch: a second launch costs
+// about 3 us, one workgroup reads about 100 GB/s.  Branches of 8 kv heads x 128: 94 blocks 7.0 us; 500 blocks 10.6 where
+// the two kernels take 9; 1000 blocks 14.8.
+constexpr size_t kSelFusedBytes = 80 << 10;    // codes of the context per kv head, with few rows
+constexpr int kSelFusedRows = 256;             // (row, kv head) pairs that keep every CU busy by themselves
+constexpr int kSelFused = 1024;                // blocks, the most that kernel takes
+constexpr int kSelShort = 128;                 // blocks up to which chunks take it too, and fewer threads do
+constexpr size_t kSelWaves = 4096, kSelTileWgs = 256;     // waves / workgroups the scores are spread over
 typedef int sel_i32x4 __attribute__((ext_vector_type(4)));
 
 struct SelArgs {
@@ -527,40 +533,57 @@ __global__ __launch_bounds__(THREADS) void topk_kernel(SelArgs A, int KVH)
     });
 }
 
-// Scores and selection of one (row, kv head) in one workgroup, for contexts of few blocks: the keys stay in LDS.
-template <int D, int THREADS>
+// Scores and selection of one (row, kv head) in one workgroup, for contexts of few blocks: the keys stay in LDS.  A wave
+// asks for the table entries, then for the codes, of up to four groups at once, so that the kernel is three round
+// trips to memory (length, table, codes) and the selection.
+template <int D, int THREADS, int BLOCKS>
 __global__ __launch_bounds__(THREADS) void select_kernel(Lay a, SelArgs A)
 {
-    constexpr int W = THREADS / 64, NR = kSelFused / THREADS, KS = D / 32;
+    constexpr int W = THREADS / 64, NR = BLOCKS / THREADS > 0 ? BLOCKS / THREADS : 1, KS = D / 32, GPW = BLOCKS / 16 / W;
+    constexpr int G = GPW < 4 ? GPW : 4;
+    static_assert(GPW * 16 * W == BLOCKS && GPW % G == 0, "whole rounds of groups");
     __shared__ TopkLds<THREADS> S;
-    __shared__ uint32_t key_lds[kSelFused];
+    __shared__ uint32_t key_lds[BLOCKS];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int t = blockIdx.x / a.KVH, h = blockIdx.x - t * a.KVH, GQ = a.QH / a.KVH;
     const int32_t *tab = A.tables + (size_t)t * A.table_stride;
-    const int nb = min(sel_blocks_of_row(A, t), kSelFused);
+    const int nb = min(sel_blocks_of_row(A, t), BLOCKS);
     const int groups = (nb + 15) / 16;
-    int blk = w * 16 + c < nb ? tab[w * 16 + c] : -1;
     sel_i32x4 qa[KS];
     const int eq = sel_query<D>(A.q + ((size_t)t * a.QH + h * GQ + min(c & (A.P - 1), GQ - 1)) * D * 2, g, A.io_dtype, qa);
     float qm[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) qm[j] = sel_pow2(__shfl(eq, 4 * g + j));
-    for (int gi = w; gi < groups; gi += W) {
-        const bool hole = blk < 0 || blk >= a.NB;
-        const size_t entry = (size_t)(hole ? 0 : blk) * a.KVH + h;          // block 0 is always mapped; its score is not used
-        const uint8_t *cp = A.bounds + entry * (2 * D) + g * 16;
-        uint4 bv[KS];
+    for (int g0 = w; g0 < groups; g0 += G * W) {
+        int blk[G], e[G];
+        uint4 bv[G][KS];
 #pragma unroll
-        for (int k = 0; k < KS; k++) bv[k] = *(const uint4 *)(cp + k * 64);
-        const int e = hole ? kNoBlock : (int)(int8_t)A.exps[entry], b = gi * 16 + c;
-        blk = b + W * 16 < nb ? tab[b + W * 16] : -1;
-        sel_i32x4 acc = {0, 0, 0, 0};
+        for (int i = 0; i < G; i++) {
+            const int b = (g0 + i * W) * 16 + c;
+            blk[i] = b < nb ? tab[b] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            if (g0 + i * W >= groups) continue;                          // the same for the whole wave
+            const bool hole = blk[i] < 0 || blk[i] >= a.NB;
+            const size_t entry = (size_t)(hole ? 0 : blk[i]) * a.KVH + h;      // block 0 is always mapped; its score is not used
+            const uint8_t *cp = A.bounds + entry * (2 * D) + g * 16;
+#pragma unroll
+            for (int k = 0; k < KS; k++) bv[i][k] = *(const uint4 *)(cp + k * 64);
+            e[i] = hole ? kNoBlock : (int)(int8_t)A.exps[entry];
+        }
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            if (g0 + i * W >= groups) continue;
+            const int b = (g0 + i * W) * 16 + c;
+            sel_i32x4 acc = {0, 0, 0, 0};
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
-        for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[k], __builtin_bit_cast(sel_i32x4, bv[k]), acc, 0, 0, 0);
+            for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[k], __builtin_bit_cast(sel_i32x4, bv[i][k]), acc, 0, 0, 0);
 #endif
-        const float x = sel_row_max(acc, qm, A.P, e == kNoBlock ? 0.0f : sel_pow2(e));
-        if (g == 0) key_lds[b] = sel_key_of(A, x, b, nb, e);
+            const float x = sel_row_max(acc, qm, A.P, e[i] == kNoBlock ? 0.0f : sel_pow2(e[i]));
+            if (g == 0) key_lds[b] = sel_key_of(A, x, b, nb, e[i]);
+        }
     }
     __syncthreads();
     uint32_t kr[NR];
@@ -635,11 +658,21 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
     const bool tile = table_stride == 0 && a.D <= 256 && T > 4 * A.R;      // more than four sets of rows over one table
     const int n = (int)(((size_t)max_seq_len + a.bs - 1) / a.bs);
     hipStream_t st = (hipStream_t)stream;
-    if (n <= kSelFused && a.D <= 256 && !tile) {
+    if (n <= kSelShort || (n <= kSelFused && a.D <= 256 && !tile &&
+                           ((size_t)n * 2 * a.D <= kSelFusedBytes || (size_t)T * a.KVH >= kSelFusedRows))) {
         const dim3 grid(T * a.KVH);
-        if (a.D == 64) hipLaunchKernelGGL((select_kernel<64, 1024>), grid, dim3(1024), 0, st, a, A);
-        else if (a.D == 128) hipLaunchKernelGGL((select_kernel<128, 1024>), grid, dim3(1024), 0, st, a, A);
-        else hipLaunchKernelGGL((select_kernel<256, 512>), grid, dim3(512), 0, st, a, A);
+#define DRK_SELECT_LAUNCH(D)                                                                                                       \
+    do {                                                                                                                           \
+        if (n <= kSelShort) hipLaunchKernelGGL((select_kernel<D, 256, kSelShort>), grid, dim3(256), 0, st, a, A);                  \
+        else hipLaunchKernelGGL((select_kernel<(D < 512 ? D : 256), 512, kSelFused>), grid, dim3(512), 0, st, a, A);               \
+    } while (0)
+        switch (a.D) {
+        case 64: DRK_SELECT_LAUNCH(64); break;
+        case 128: DRK_SELECT_LAUNCH(128); break;
+        case 256: DRK_SELECT_LAUNCH(256); break;
+        default: DRK_SELECT_LAUNCH(512); break;                      // short contexts only
+        }
+#undef DRK_SELECT_LAUNCH
         DRK_LAUNCH_CHECK("select_kernel");
         return DRK_OK;
     }
@@ -648,10 +681,10 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
         const size_t tiles = ((size_t)T + rows - 1) / rows, groups = ((size_t)n + 15) / 16;
         if (tiles > 65535 || groups > 65535) return fail(DRK_ERR_UNSUPPORTED, "block_select: %d rows are more than one launch takes", T);
         const size_t all = groups * a.KVH * tiles;                        // 16-block groups of every kv head and row tile
-        const size_t units = tile ? kSelTileWgs : kSelWaves;              // as many as should have work of their own
+        const size_t units = tile ? kSelTileWgs : (a.D <= 128 ? kSelWaves : kSelWaves / 2);              // as many as should have work of their own
         const size_t gpw = (all + units - 1) / units;
-        A.groups_per_wave = (int)(gpw > 32 ? 32 : gpw);
-        if (tile) A.groups_per_wave = (int)((gpw + 1) & ~(size_t)1);
+        // a wave's first load covers the table entries of four groups: 16 branches x 64k, 4 groups 33.5 us, 8 groups 35.7
+        A.groups_per_wave = (int)(tile ? ((gpw > 32 ? 32 : gpw) + 1) & ~(size_t)1 : (gpw > 4 ? 4 : gpw));
         const size_t per = (size_t)A.groups_per_wave * (tile ? 1 : 4);
         const dim3 grid(a.KVH, (unsigned)((groups + per - 1) / per), (unsigned)tiles);
         switch (a.D) {

@@ -16,8 +16,9 @@ namespace drk {
 
 constexpr int kSpGroups = 512;          // 16-token groups one workgroup may own (descriptors in LDS)
 constexpr int kSpMaxPieces = 64;        // pieces of a row: a lane each in the merge
-constexpr int kSpWaves = 8;
-constexpr int kSpWgs = 512;             // workgroups a launch aims at: 2 per CU
+constexpr int kSpWaves = 8;             // waves of a workgroup
+constexpr size_t kSpUncut = 32 * 128;   // groups times head_dim up to which a row is not cut
+constexpr int kSpWgs = 512;             // workgroups of head_dim 128 a launch aims at: the 2 a CU holds (head_dim 256: half)
 
 struct SparseArgs {
     const uint8_t *pool_layer, *q;
@@ -429,14 +430,18 @@ __global__ __launch_bounds__(64) void sparse_merge_kernel(SparseArgs A)
     }
 }
 
-// Pieces of a (row, kv head): enough workgroups for the chip, but no piece shorter than a group per wave
-// and none longer than the descriptor table.
+// Pieces of a (row, kv head): enough workgroups for the chip, but no piece shorter than a group per wave and none
+// longer than the descriptor table.  A cut costs a second launch and the merge, about 3 us, so a short list is walked
+// by one workgroup: one row of 8 kv heads x 128, 32 groups each, 9.3 us instead of 10.5 -- but 64 groups 16 instead
+// of 10 (with 16 waves in the workgroup), and at head_dim 256, whose groups are twice the bytes, 32 groups 15.5
+// instead of 11.6.
 static int sparse_pieces(const Lay &a, int T, int n_keep, int *groups_per_piece)
 {
     const size_t groups = (size_t)n_keep * (a.bs / 16), rows = (size_t)T * a.KVH;
-    size_t p = (kSpWgs + rows - 1) / rows;
+    size_t p = (kSpWgs * 128 / a.D + rows - 1) / rows;
     p = p > (groups + kSpWaves - 1) / kSpWaves ? (groups + kSpWaves - 1) / kSpWaves : p;
     p = p > kSpMaxPieces ? kSpMaxPieces : p;
+    if (groups * a.D <= kSpUncut) p = 1;
     const size_t least = (groups + kSpGroups - 1) / kSpGroups;
     p = p < least ? least : p;
     if (p > kSpMaxPieces) return 0;
@@ -532,13 +537,14 @@ int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void
     hipStream_t st = (hipStream_t)stream;
     const bool shared = table_stride == 0 && T > 1;           // rows over one table meet in the same pages: keep them cached
     const int wpr = A.pieces > 1 ? 8 : sparse_waves_per_row(a, T, A.groups_per_piece);
-    const dim3 grid((unsigned)(((size_t)T * wpr + 7) / 8 * A.pieces * a.KVH));
+    const int per_wg = kSpWaves / wpr;                        // rows of a workgroup
+    const dim3 grid((unsigned)(((size_t)T + per_wg - 1) / per_wg * A.pieces * a.KVH));
 #define DRK_SPARSE_LAUNCH4(DT, D, NT, WPR)                                                                                  \
-    hipLaunchKernelGGL((sparse_kernel<DT, D, NT, WPR>), grid, dim3(kSpWaves * 64),                                          \
-                       sparse_lds(a.QH / a.KVH, StreamGeo<DT, D>::PITCH, A.groups_per_piece, DT == DRK_INT8, 8 / WPR).total, st, A)
+    hipLaunchKernelGGL((sparse_kernel<DT, D, NT, WPR>), grid, dim3(kSpWaves * 64),                              \
+                       sparse_lds(a.QH / a.KVH, StreamGeo<DT, D>::PITCH, A.groups_per_piece, DT == DRK_INT8, per_wg).total, st, A)
 #define DRK_SPARSE_LAUNCH3(DT, D, NT)                                                                                       \
     do {                                                                                                                    \
-        if (wpr == 8) DRK_SPARSE_LAUNCH4(DT, D, NT, 8);                                                                     \
+        if (wpr == 8) DRK_SPARSE_LAUNCH4(DT, D, NT, 8);                                                                \
         else if (wpr == 4) DRK_SPARSE_LAUNCH4(DT, D, NT, 4);                                                                \
         else if (wpr == 2) DRK_SPARSE_LAUNCH4(DT, D, NT, 2);                                                                \
         else DRK_SPARSE_LAUNCH4(DT, D, NT, 1);                                                                              \

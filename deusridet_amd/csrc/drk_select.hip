@@ -58,21 +58,67 @@ __device__ __forceinline__ int sel_blocks_of_row(const SelArgs &A, int t)
 __device__ __forceinline__ uint32_t sel_key(float s)
 {
     const uint32_t u = __float_as_uint(s);
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
 }
 
+__device__ __forceinline__ float sel_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
 // ---- query heads as an operand ----------------------------------------------------------------------
+// four codes (the low bytes of u) as one dword, split into its negative and its positive bytes
+__device__ __forceinline__ void sel_split4(const uint32_t (&u)[4], uint32_t &neg, uint32_t &pos)
+{
+    const uint32_t c = s_perm(s_perm(u[3], u[2], 0x04000c0cu), s_perm(u[1], u[0], 0x0c0c0400u), 0x07060100u);
+    const uint32_t s = (c >> 7) & 0x01010101u, mask = (s << 8) - s;             // 0xff in the negative codes' bytes
+    neg = c & mask;
+    pos = c & ~mask;
+}
+
 // Codes c = rint(q 2^-eq) of one head row; lane (c, g) holds dims 64 k + 16 g .. + 15: the negative parts meet the
-// lows (first D / 64 steps), the positive parts the highs.
+// lows (first D / 64 steps), the positive parts the highs.  Adding 1.5 * 2^23 to x * 2^-e in one fused operation rounds to
+// the nearest whole number, ties to even, and leaves the code as the low byte: the product is exact and at most 127.
+// Rows with a NaN, or beyond the exponents' range, take the long way.
 template <int D>
 __device__ __forceinline__ int sel_query(const uint8_t *row, int g, int io_dtype, sel_i32x4 *qa)
 {
     constexpr int HK = D / 64;
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
     uint4 raw[HK][2];
 #pragma unroll
     for (int k = 0; k < HK; k++) {
         raw[k][0] = *(const uint4 *)(row + k * 128 + g * 32);
         raw[k][1] = *(const uint4 *)(row + k * 128 + g * 32 + 16);
+    }
+    u16x2 m2 = {0, 0};                                                          // magnitudes order like their bits
+#pragma unroll
+    for (int k = 0; k < HK; k++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const uint32_t w[4] = {raw[k][j].x, raw[k][j].y, raw[k][j].z, raw[k][j].w};
+#pragma unroll
+            for (int i = 0; i < 4; i++) m2 = __builtin_elementwise_max(m2, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
+        }
+    int m = max((int)m2.x, (int)m2.y);
+    m = max(m, __shfl_xor(m, 16));
+    m = max(m, __shfl_xor(m, 32));
+    int e = bounds_exponent(elem16_to_f((uint16_t)m, io_dtype));
+    if (__ballot(m > (io_dtype == DRK_BF16 ? 0x7f80 : 0x7c00) || e == 40) == 0) {
+        const float inv = sel_pow2(-e);
+#pragma unroll
+        for (int k = 0; k < HK; k++) {
+            uint32_t n[4], p[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                float x[8];
+                uint32_t u[4];
+                unpack8(raw[k][j >> 1], io_dtype, x);
+#pragma unroll
+                for (int i = 0; i < 4; i++) u[i] = __float_as_uint(__fmaf_rn(x[4 * (j & 1) + i], inv, 12582912.0f));
+                sel_split4(u, n[j], p[j]);
+            }
+            qa[k] = sel_i32x4{(int)n[0], (int)n[1], (int)n[2], (int)n[3]};
+            qa[HK + k] = sel_i32x4{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
+        }
+        return e;
     }
     float amax = 0.0f;
 #pragma unroll
@@ -86,8 +132,8 @@ __device__ __forceinline__ int sel_query(const uint8_t *row, int g, int io_dtype
         }
     amax = fmaxf(amax, __shfl_xor(amax, 16));
     amax = fmaxf(amax, __shfl_xor(amax, 32));
-    const int e = bounds_exponent(amax);
-    const float inv = ldexpf(1.0f, -e);
+    e = bounds_exponent(amax);
+    const float inv = sel_pow2(-e);
 #pragma unroll
     for (int k = 0; k < HK; k++) {
         uint32_t n[4], p[4];
@@ -98,14 +144,10 @@ __device__ __forceinline__ int sel_query(const uint8_t *row, int g, int io_dtype
             unpack8(raw[k][j >> 1], io_dtype, x);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                float y = x[4 * (j & 1) + i] * inv;
-                y = fminf(fmaxf(y == y ? y : 0.0f, -127.0f), 127.0f);
-                u[i] = __float_as_uint(__fadd_rn(y, 12582912.0f));              // 1.5 * 2^23: rounds to even, the code is the low byte
+                const float y = x[4 * (j & 1) + i] * inv;
+                u[i] = __float_as_uint(__fadd_rn(fminf(fmaxf(y == y ? y : 0.0f, -127.0f), 127.0f), 12582912.0f));
             }
-            const uint32_t c = s_perm(s_perm(u[3], u[2], 0x04000c0cu), s_perm(u[1], u[0], 0x0c0c0400u), 0x07060100u);
-            const uint32_t s = (c >> 7) & 0x01010101u, mask = (s << 8) - s;     // 0xff in the negative codes' bytes
-            n[j] = c & mask;
-            p[j] = c & ~mask;
+            sel_split4(u, n[j], p[j]);
         }
         qa[k] = sel_i32x4{(int)n[0], (int)n[1], (int)n[2], (int)n[3]};
         qa[HK + k] = sel_i32x4{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
@@ -113,33 +155,37 @@ __device__ __forceinline__ int sel_query(const uint8_t *row, int g, int io_dtype
     return e;
 }
 
-__device__ __forceinline__ float sel_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-
-// Heads 4g + j of one product against block c: the largest score over the P heads of a row (P = 4, 8 or 16), valid in every
-// lane of the row.  qm = 2^eq of the heads, bm = 2^e of the block.
-__device__ __forceinline__ float sel_row_max(const sel_i32x4 &acc, const float *qm, int P, float bm)
+// Heads 4g + j of one product against block c: the key of the largest score over the P heads of a row (P = 4, 8 or 16), in
+// every lane of the row.  qm = 2^eq of the heads, bm = 2^e of the block.  A row's other heads are 16 (and 32) lanes
+// away: the two results of a swap with itself are the two sides.
+template <int P>
+__device__ __forceinline__ uint32_t sel_row_key(const sel_i32x4 &acc, const float *qm, float bm)
 {
-    float x = fmaxf(fmaxf((float)acc[0] * qm[0], (float)acc[1] * qm[1]), fmaxf((float)acc[2] * qm[2], (float)acc[3] * qm[3]));
+    const float x = fmaxf(fmaxf((float)acc[0] * qm[0], (float)acc[1] * qm[1]), fmaxf((float)acc[2] * qm[2], (float)acc[3] * qm[3]));
+    uint32_t k = sel_key(x * bm);
 #if defined(__HIP_DEVICE_COMPILE__)
-    // a row's other heads are 16 (and 32) lanes away: the two results of a swap with itself are the two sides
-    if (P >= 8) {
-        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    if constexpr (P >= 8) {
+        const auto s = __builtin_amdgcn_permlane16_swap(k, k, false, false);
+        k = max((uint32_t)s[0], (uint32_t)s[1]);
     }
-    if (P >= 16) {
-        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    if constexpr (P >= 16) {
+        const auto s = __builtin_amdgcn_permlane32_swap(k, k, false, false);
+        k = max((uint32_t)s[0], (uint32_t)s[1]);
     }
 #endif
-    return x * bm;
+    return k;
+}
+__device__ __forceinline__ uint32_t sel_row_key(const sel_i32x4 &acc, const float *qm, int P, float bm)
+{
+    return P == 4 ? sel_row_key<4>(acc, qm, bm) : (P == 8 ? sel_row_key<8>(acc, qm, bm) : sel_row_key<16>(acc, qm, bm));
 }
 
 constexpr int kNoBlock = 1000;          // in place of the exponent of a block without a page
 
-__device__ __forceinline__ uint32_t sel_key_of(const SelArgs &A, float x, int b, int nb, int e)
+__device__ __forceinline__ uint32_t sel_key_of(const SelArgs &A, uint32_t scored, int b, int nb, int e)
 {
-    if (b >= nb || e == kNoBlock) return 0u;
-    return b < A.sink || b >= nb - A.recent ? kKeyForced : sel_key(x);
+    const bool forced = (b < A.sink) | (b >= nb - A.recent), none = (b >= nb) | (e == kNoBlock);
+    return none ? 0u : (forced ? kKeyForced : scored);
 }
 
 // One set of 16 heads per wave: a branch's row (R = 1), or R = 16 / P rows of one table.
@@ -193,7 +239,7 @@ __global__ __launch_bounds__(256) void score_kernel(Lay a, SelArgs A)
             }
             fetch(i + 1);
         }
-        const float x = sel_row_max(acc, qm, A.P, e == kNoBlock ? 0.0f : sel_pow2(e));
+        const uint32_t x = sel_row_key(acc, qm, A.P, e == kNoBlock ? 0.0f : sel_pow2(e));
         const int b = (first + i) * 16 + c;
         if ((A.R > 1 ? ((4 * g) & (A.P - 1)) == 0 : g == 0) && row < A.T && (unsigned)b < A.key_stride)
             A.keys[((size_t)row * a.KVH + h) * A.key_stride + b] = sel_key_of(A, x, b, nbr, e);
@@ -203,19 +249,20 @@ __global__ __launch_bounds__(256) void score_kernel(Lay a, SelArgs A)
 // Rows of one table.  A workgroup's 8 waves hold SETS sets of 16 heads each (8 SETS R rows together) and walk the same
 // blocks, 32 at a time, whose codes the workgroup stages in LDS, two buffers by turns, requested two steps ahead: every
 // byte of the bounds is read once per 8 SETS R rows.
-template <int D, int SETS>
+template <int D, int SETS, int P>
 __global__ __launch_bounds__(512) void score_tile_kernel(Lay a, SelArgs A)
 {
     constexpr int KS = D / 32, CH = 2 * D / 16;              // 16-byte chunks of a block's codes
+    constexpr int R = 16 / P;                                // rows per set
     constexpr int PITCH = 2 * D + 16, G = 2, PER = (16 * G * CH + 511) / 512;
     static_assert(512 % CH == 0, "a thread's chunks are the same one of several blocks");
     __shared__ __align__(16) uint8_t b_lds[2][16 * G * PITCH];
     __shared__ int e_lds[2][16 * G];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int h = blockIdx.x, GQ = a.QH / a.KVH;
-    const int row0 = (int)blockIdx.z * (8 * SETS * A.R), wrow0 = row0 + w * SETS * A.R;
+    const int row0 = (int)blockIdx.z * (8 * SETS * R), wrow0 = row0 + w * SETS * R;
     const int first = (int)blockIdx.y * A.groups_per_wave;   // 16-block groups; a workgroup takes an even number
-    const int last_row = min(row0 + 8 * SETS * A.R, A.T) - 1;
+    const int last_row = min(row0 + 8 * SETS * R, A.T) - 1;
     // lengths may be any where they are given: the workgroup walks to its longest row
     int nbmax = 0;
     for (int r = row0 + lane; r <= last_row; r += 64) nbmax = max(nbmax, sel_blocks_of_row(A, r));
@@ -260,17 +307,25 @@ __global__ __launch_bounds__(512) void score_tile_kernel(Lay a, SelArgs A)
     sel_i32x4 qa[SETS][KS];
     float qm[SETS][4];
     int nbr[SETS];
-    uint32_t *kp[SETS];
+    unsigned ko[SETS];                                       // keys of the lane's rows, counted from the workgroup's first row
+    bool on[SETS];
+    uint32_t *const kbase = A.keys + ((size_t)row0 * a.KVH + h) * A.key_stride;
+    int nbmin = 0x7fffffff;
 #pragma unroll
     for (int s = 0; s < SETS; s++) {
-        const int qrow = min(wrow0 + s * A.R + c / A.P, A.T - 1);
-        const int eq = sel_query<D>(A.q + ((size_t)qrow * a.QH + h * GQ + min(c & (A.P - 1), GQ - 1)) * D * 2, g, A.io_dtype, qa[s]);
+        const int qrow = min(wrow0 + s * R + c / P, A.T - 1);
+        const int eq = sel_query<D>(A.q + ((size_t)qrow * a.QH + h * GQ + min(c & (P - 1), GQ - 1)) * D * 2, g, A.io_dtype, qa[s]);
 #pragma unroll
         for (int j = 0; j < 4; j++) qm[s][j] = sel_pow2(__shfl(eq, 4 * g + j));
-        const int row = wrow0 + s * A.R + 4 * g / A.P;
+        const int row = wrow0 + s * R + 4 * g / P;
         nbr[s] = row < A.T ? sel_blocks_of_row(A, row) : 0;
-        kp[s] = ((4 * g) & (A.P - 1)) == 0 && row < A.T ? A.keys + ((size_t)row * a.KVH + h) * A.key_stride : nullptr;
+        on[s] = ((4 * g) & (P - 1)) == 0 && row < A.T;
+        ko[s] = (unsigned)(row - row0) * (unsigned)a.KVH * A.key_stride;
+        nbmin = min(nbmin, nbr[s]);
     }
+#pragma unroll
+    for (int off = 16; off < 64; off <<= 1) nbmin = min(nbmin, __shfl_xor(nbmin, off));
+    const int scored_end = __builtin_amdgcn_readfirstlane(nbmin) - A.recent;    // from the first blocks to here every row only scores
     fetch(1);
     page(2);
     stage(0);
@@ -279,24 +334,42 @@ __global__ __launch_bounds__(512) void score_tile_kernel(Lay a, SelArgs A)
         fetch(1);
         page(i + 3);
         const uint8_t *buf = b_lds[i & 1];
+        uint4 bv[G][KS];
+#pragma unroll
+        for (int x = 0; x < G; x++)
+#pragma unroll
+            for (int k = 0; k < KS; k++) bv[x][k] = *(const uint4 *)(buf + (x * 16 + c) * PITCH + k * 64 + g * 16);
+        // G * SETS chains of products side by side, then what becomes of them
+        sel_i32x4 acc[G][SETS];
+#pragma unroll
+        for (int k = 0; k < KS; k++)
+#pragma unroll
+            for (int x = 0; x < G; x++)
+#pragma unroll
+                for (int s = 0; s < SETS; s++) {
+                    if (k == 0) acc[x][s] = sel_i32x4{0, 0, 0, 0};
+#if defined(__HIP_DEVICE_COMPILE__)
+                    acc[x][s] = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[s][k], __builtin_bit_cast(sel_i32x4, bv[x][k]), acc[x][s], 0, 0, 0);
+#endif
+                }
 #pragma unroll
         for (int x = 0; x < G; x++) {
-            uint4 bv[KS];
+            const int e = e_lds[i & 1][x * 16 + c], b0 = (first + i * G + x) * 16, b = b0 + c;
+            const bool hole = e == kNoBlock, inner = b0 >= A.sink && b0 + 16 <= scored_end;
+            const float bm = hole ? 0.0f : sel_pow2(e);
+            uint32_t key[SETS];
 #pragma unroll
-            for (int k = 0; k < KS; k++) bv[k] = *(const uint4 *)(buf + (x * 16 + c) * PITCH + k * 64 + g * 16);
-            const int e = e_lds[i & 1][x * 16 + c], b = (first + i * G + x) * 16 + c;
-            const float bm = e == kNoBlock ? 0.0f : sel_pow2(e);
+            for (int s = 0; s < SETS; s++) key[s] = hole ? 0u : sel_row_key<P>(acc[x][s], qm[s], bm);
+            if (!inner) {                                    // the same for the whole wave
 #pragma unroll
-            for (int s = 0; s < SETS; s++) {
-                sel_i32x4 acc = {0, 0, 0, 0};
-#if defined(__HIP_DEVICE_COMPILE__)
-#pragma unroll
-                for (int k = 0; k < KS; k++)
-                    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[s][k], __builtin_bit_cast(sel_i32x4, bv[k]), acc, 0, 0, 0);
-#endif
-                const float y = sel_row_max(acc, qm[s], A.P, bm);
-                if (kp[s] && (unsigned)b < A.key_stride) kp[s][b] = sel_key_of(A, y, b, nbr[s], e);
+                for (int s = 0; s < SETS; s++) {
+                    const bool forced = (b < A.sink) | (b >= nbr[s] - A.recent);
+                    key[s] = (b >= nbr[s] || hole) ? 0u : (forced ? kKeyForced : key[s]);
+                }
             }
+#pragma unroll
+            for (int s = 0; s < SETS; s++)
+                if (on[s] & ((unsigned)b < A.key_stride)) kbase[ko[s] + (unsigned)b] = key[s];
         }
         stage((i + 1) & 1);
         __syncthreads();
@@ -581,7 +654,7 @@ __global__ __launch_bounds__(THREADS) void select_kernel(Lay a, SelArgs A)
 #pragma unroll
             for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[k], __builtin_bit_cast(sel_i32x4, bv[i][k]), acc, 0, 0, 0);
 #endif
-            const float x = sel_row_max(acc, qm, A.P, e[i] == kNoBlock ? 0.0f : sel_pow2(e[i]));
+            const uint32_t x = sel_row_key(acc, qm, A.P, e[i] == kNoBlock ? 0.0f : sel_pow2(e[i]));
             if (g == 0) key_lds[b] = sel_key_of(A, x, b, nb, e[i]);
         }
     }
@@ -604,7 +677,12 @@ template <int D>
 static void launch_score(const Lay &a, const SelArgs &A, bool tile, dim3 grid, hipStream_t st)
 {
     if constexpr (D <= 256) {
-        if (tile) { hipLaunchKernelGGL((score_tile_kernel<D, 2>), grid, dim3(512), 0, st, a, A); return; }
+        if (tile) {
+            if (A.P == 4) hipLaunchKernelGGL((score_tile_kernel<D, 2, 4>), grid, dim3(512), 0, st, a, A);
+            else if (A.P == 8) hipLaunchKernelGGL((score_tile_kernel<D, 2, 8>), grid, dim3(512), 0, st, a, A);
+            else hipLaunchKernelGGL((score_tile_kernel<D, 2, 16>), grid, dim3(512), 0, st, a, A);
+            return;
+        }
     }
     hipLaunchKernelGGL((score_kernel<D>), grid, dim3(256), 0, st, a, A);
 }
@@ -655,7 +733,8 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
     A.P = 4;
     while (A.P < a.QH / a.KVH) A.P *= 2;
     A.R = table_stride == 0 && T > 1 ? 16 / A.P : 1;
-    const bool tile = table_stride == 0 && a.D <= 256 && T > 4 * A.R;      // more than four sets of rows over one table
+    // more than four sets of rows over one table; its keys are counted in 32 bits over the 64 rows of a workgroup
+    const bool tile = table_stride == 0 && a.D <= 256 && T > 4 * A.R && (size_t)a.KVH * A.key_stride <= (1u << 26);
     const int n = (int)(((size_t)max_seq_len + a.bs - 1) / a.bs);
     hipStream_t st = (hipStream_t)stream;
     if (n <= kSelShort || (n <= kSelFused && a.D <= 256 && !tile &&

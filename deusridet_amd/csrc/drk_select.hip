@@ -64,13 +64,40 @@ __device__ __forceinline__ uint32_t sel_key(float s)
 __device__ __forceinline__ float sel_pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // ---- query heads as an operand ----------------------------------------------------------------------
-// four codes (the low bytes of u) as one dword, split into its negative and its positive bytes
+// Four codes (the low bytes of u = 1.5 * 2^23 + c) as one dword, split into its negative and its positive bytes: the byte
+// above a code is 0xff where the code is negative and 0 elsewhere.
 __device__ __forceinline__ void sel_split4(const uint32_t (&u)[4], uint32_t &neg, uint32_t &pos)
 {
-    const uint32_t c = s_perm(s_perm(u[3], u[2], 0x04000c0cu), s_perm(u[1], u[0], 0x0c0c0400u), 0x07060100u);
-    const uint32_t s = (c >> 7) & 0x01010101u, mask = (s << 8) - s;             // 0xff in the negative codes' bytes
+    const uint32_t a = s_perm(u[1], u[0], 0x05010400u), b = s_perm(u[3], u[2], 0x05010400u);
+    const uint32_t c = s_perm(b, a, 0x05040100u), mask = s_perm(b, a, 0x07060302u);
     neg = c & mask;
     pos = c & ~mask;
+}
+
+// x 2^-e rounded to the nearest whole number, as sel_split4 takes it, of the HK * 16 dims of a lane
+template <int HK, bool BF16>
+__device__ __forceinline__ void sel_codes(const uint4 (&raw)[HK][2], float inv, sel_i32x4 *qa)
+{
+#pragma unroll
+    for (int k = 0; k < HK; k++) {
+        uint32_t n[4], p[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint4 &r = raw[k][j >> 1];
+            const uint32_t w[2] = {j & 1 ? r.z : r.x, j & 1 ? r.w : r.y};
+            uint32_t u[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                float x;
+                if constexpr (BF16) x = __uint_as_float(i & 1 ? w[i >> 1] & 0xffff0000u : w[i >> 1] << 16);
+                else x = (float)__builtin_bit_cast(_Float16, (uint16_t)(i & 1 ? w[i >> 1] >> 16 : w[i >> 1]));
+                u[i] = __float_as_uint(__builtin_fmaf(x, inv, 12582912.0f));
+            }
+            sel_split4(u, n[j], p[j]);
+        }
+        qa[k] = sel_i32x4{(int)n[0], (int)n[1], (int)n[2], (int)n[3]};
+        qa[HK + k] = sel_i32x4{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
+    }
 }
 
 // Codes c = rint(q 2^-eq) of one head row; lane (c, g) holds dims 64 k + 16 g .. + 15: the negative parts meet the
@@ -102,22 +129,8 @@ __device__ __forceinline__ int sel_query(const uint8_t *row, int g, int io_dtype
     m = max(m, __shfl_xor(m, 32));
     int e = bounds_exponent(elem16_to_f((uint16_t)m, io_dtype));
     if (__ballot(m > (io_dtype == DRK_BF16 ? 0x7f80 : 0x7c00) || e == 40) == 0) {
-        const float inv = sel_pow2(-e);
-#pragma unroll
-        for (int k = 0; k < HK; k++) {
-            uint32_t n[4], p[4];
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float x[8];
-                uint32_t u[4];
-                unpack8(raw[k][j >> 1], io_dtype, x);
-#pragma unroll
-                for (int i = 0; i < 4; i++) u[i] = __float_as_uint(__fmaf_rn(x[4 * (j & 1) + i], inv, 12582912.0f));
-                sel_split4(u, n[j], p[j]);
-            }
-            qa[k] = sel_i32x4{(int)n[0], (int)n[1], (int)n[2], (int)n[3]};
-            qa[HK + k] = sel_i32x4{(int)p[0], (int)p[1], (int)p[2], (int)p[3]};
-        }
+        if (io_dtype == DRK_BF16) sel_codes<HK, true>(raw, sel_pow2(-e), qa);
+        else sel_codes<HK, false>(raw, sel_pow2(-e), qa);
         return e;
     }
     float amax = 0.0f;

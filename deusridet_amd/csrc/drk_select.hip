@@ -32,7 +32,9 @@ constexpr size_t kSelFusedBytes = 80 << 10;    // codes of the context per kv he
 constexpr int kSelFusedRows = 256;             // (row, kv head) pairs that keep every CU busy by themselves
 constexpr int kSelFused = 1024;                // blocks, the most that kernel takes
 constexpr int kSelShort = 128;                 // blocks up to which chunks take it too, and fewer threads do
-constexpr size_t kSelWaves = 4096, kSelTileWgs = 256;     // waves / workgroups the scores are spread over
+constexpr size_t kSelWaves = 4096;             // waves that a decode step's scores are spread over
+constexpr unsigned kSelTileWgs = 256;          // CUs that a chunk's workgroups are spread over
+constexpr unsigned kSelTileStart = 6;          // what such a workgroup spends on its queries, counted in groups
 typedef int sel_i32x4 __attribute__((ext_vector_type(4)));
 
 struct SelArgs {
@@ -686,6 +688,24 @@ static unsigned sel_key_stride(const Lay &a, int max_seq_len)
     return (unsigned)(((size_t)max_seq_len + a.bs - 1) / a.bs + 3) & ~3u;
 }
 
+// Groups a workgroup of score_tile_kernel walks.  `rows` workgroups stand side by side; the context is cut into the number
+// of parts that ends soonest: workgroups per CU, times a part's groups and its queries' conversion.  At head_dim 256 a CU holds
+// one workgroup, below two and more, whose loads and products overlap by about a fifth; there a part is at most 64 groups
+// (1 MiB of codes), so that the rows' workgroups stay near each other in the cache.  Against about 256 workgroups of at most 32 groups
+// each: 1024 tokens x 4 heads x 256 at 16k 74 -> 51 us, 2048 tokens at 64k 343 -> 296 us.
+static int sel_tile_groups(const Lay &a, unsigned groups, unsigned rows)
+{
+    const unsigned least = a.D <= 128 ? (groups + 63) / 64 : 1;
+    unsigned best = 0xffffffffu, take = 2;
+    for (unsigned parts = least; parts == least || (parts <= groups && rows * parts <= 4 * kSelTileWgs); parts++) {
+        const unsigned g = ((groups + parts - 1) / parts + 1) & ~1u;
+        const unsigned per_cu = (rows * ((groups + g - 1) / g) + kSelTileWgs - 1) / kSelTileWgs;
+        const unsigned cost = (a.D <= 128 && per_cu > 1 ? 4 : 5) * per_cu * (g + kSelTileStart);
+        if (cost < best) { best = cost; take = g; }
+    }
+    return (int)take;
+}
+
 template <int D>
 static void launch_score(const Lay &a, const SelArgs &A, bool tile, dim3 grid, hipStream_t st)
 {
@@ -773,10 +793,14 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
         const size_t tiles = ((size_t)T + rows - 1) / rows, groups = ((size_t)n + 15) / 16;
         if (tiles > 65535 || groups > 65535) return fail(DRK_ERR_UNSUPPORTED, "block_select: %d rows are more than one launch takes", T);
         const size_t all = groups * a.KVH * tiles;                        // 16-block groups of every kv head and row tile
-        const size_t units = tile ? kSelTileWgs : (a.D <= 128 ? kSelWaves : kSelWaves / 2);              // as many as should have work of their own
-        const size_t gpw = (all + units - 1) / units;
-        // a wave's first load covers the table entries of four groups: 16 branches x 64k, 4 groups 33.5 us, 8 groups 35.7
-        A.groups_per_wave = (int)(tile ? ((gpw > 32 ? 32 : gpw) + 1) & ~(size_t)1 : (gpw > 4 ? 4 : gpw));
+        if (tile) {
+            A.groups_per_wave = sel_tile_groups(a, (unsigned)groups, (unsigned)(tiles * a.KVH));
+        } else {
+            const size_t units = a.D <= 128 ? kSelWaves : kSelWaves / 2;          // as many waves as should have work of their own
+            const size_t gpw = (all + units - 1) / units;
+            // a wave's first load covers the table entries of four groups: 16 branches x 64k, 4 groups 33.5 us, 8 groups 35.7
+            A.groups_per_wave = (int)(gpw > 4 ? 4 : gpw);
+        }
         const size_t per = (size_t)A.groups_per_wave * (tile ? 1 : 4);
         const dim3 grid(a.KVH, (unsigned)((groups + per - 1) / per), (unsigned)tiles);
         switch (a.D) {

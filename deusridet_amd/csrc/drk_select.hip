@@ -757,6 +757,10 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
     if (need && (!workspace || workspace_bytes < need))
         return fail(DRK_ERR_WORKSPACE, "block_select: %zu bytes of workspace, %zu needed", workspace_bytes, need);
     if ((size_t)T * a.KVH > 0x7fffffffu) return fail(DRK_ERR_INVALID, "block_select: too many rows");
+    if (table_stride > 0 && (size_t)table_stride * a.bs < (size_t)max_seq_len) {        // no row is longer than its table
+        max_seq_len = table_stride * a.bs;
+        A.key_stride = sel_key_stride(a, max_seq_len);
+    }
     A.bounds = (const uint8_t *)bounds + (size_t)layer * a.NB * a.KVH * 2 * a.D;
     A.exps = (const uint8_t *)bounds + bounds_exps_offset(a) + (size_t)layer * a.NB * a.KVH;
     A.q = (const uint8_t *)q; A.tables = d_tables; A.seq_lens = d_seq_lens; A.keys = (uint32_t *)workspace; A.out = d_selected;

@@ -27,7 +27,7 @@ struct SparseArgs {
     uint16_t *out;
     float *part_o, *part_m, *part_l;     // [T][QH][pieces]([D])
     size_t gate_stride;
-    int table_stride, pos_start, T, KVH, QH, NB, bs, keep, io_dtype;
+    int table_stride, table_blocks, pos_start, T, KVH, QH, NB, bs, keep, io_dtype;
     int pieces, groups_per_piece, groups;    // 16-token groups of a (row, kv head)'s list
     unsigned head_stride, kv_plane, block_stride, scale_plane, row_bytes;
     float scale_log2e;
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel
         int cnt = 0;
         if (i0 + rtid < gn && len > 0) {
             const int e = gi / gpb, lb = sel[e], p0 = (gi - e * gpb) * 16;
-            if (lb >= 0 && lb <= (len - 1) / A.bs) {
+            if (lb >= 0 && lb <= (len - 1) / A.bs && lb < A.table_blocks) {
                 cnt = min(16, len - lb * A.bs - p0);
                 if (cnt > 0) {
                     const int blk = tab[lb];
@@ -529,7 +529,7 @@ int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void
     A.gate = (const uint16_t *)gate; A.gate_stride = gate_stride; A.out = (uint16_t *)out;
     const size_t np = (size_t)T * a.QH * A.pieces;
     A.part_o = (float *)workspace; A.part_m = A.part_o + np * a.D; A.part_l = A.part_m + np;
-    A.table_stride = table_stride; A.pos_start = pos_start; A.T = T; A.KVH = a.KVH; A.QH = a.QH; A.NB = a.NB; A.bs = a.bs;
+    A.table_stride = table_stride; A.table_blocks = table_stride > 0 ? table_stride : 0x7fffffff; A.pos_start = pos_start; A.T = T; A.KVH = a.KVH; A.QH = a.QH; A.NB = a.NB; A.bs = a.bs;
     A.keep = n_keep; A.io_dtype = io_dtype; A.groups = n_keep * (a.bs / 16);
     A.head_stride = a.head_stride; A.kv_plane = a.kv_plane; A.block_stride = a.block_stride; A.scale_plane = a.scale_plane;
     A.row_bytes = a.row_bytes;

@@ -492,7 +492,8 @@ int drk_rope_freqs_fill(const drk_rope *r, double *d_freqs, void *stream);
 int drk_rope_table_fill_scaled(const drk_rope *r, float *d_table, int n_pos, void *stream);
 /* One tensor of head rows: element (t, head, d) at t * token_stride + head * head_stride + d; strides in elements,
  * multiples of 8, pointers 16-byte aligned.  out may equal x with the same strides (in place); otherwise the two must
- * not overlap. */
+ * not overlap.  Rows of out must not overlap either, nor the out of two tensors of a call: tokens lie behind one
+ * another's heads or heads behind one another's tokens. */
 typedef struct drk_rope_rows {
     const void *x;
     void *out;
@@ -527,8 +528,8 @@ size_t drk_kv_bounds_bytes(const drk_kv_layout *g);
  * d_pos != NULL: one token for each of n branches, at d_pos[i] of table row i -- the block of d_pos[i] is covered up to
  * d_pos[i] (a negative position or a missing page is skipped).  NULL: tokens [pos_start, pos_start + n) of one table --
  * their blocks, up to pos_start + n - 1.  Tokens before pos_start in the first block count: the block is recomputed,
- * not added to, so copies made on write, reused pages and rewritten positions need nothing special.  Two branches
- * whose positions lie in the same physical block (they must not both write it) leave it covered up to one of them. */
+ * not added to, so copies made on write, reused pages and rewritten positions need nothing special.  Two branches at
+ * different positions of one physical block, which the append does not allow either, leave its bounds undefined. */
 int drk_kv_bounds_update(const drk_kv_layout *g, const void *pool, const int32_t *d_tables, int table_stride,
                          const int32_t *d_pos, int pos_start, int n, int layer, int layer_count, void *bounds,
                          void *stream);
@@ -546,8 +547,8 @@ int drk_kv_bounds_extract(const drk_kv_layout *g, void *d_dst, const void *bound
  *   2^(eq + e) * sum_d max(c_d * low_d, c_d * high_d),   c_d = rint(q_d / 2^eq),  eq as e above from max |q_d|
  * -- (up to the rounding of q) an upper bound of every logit the block can give.  It is a whole number below 2^24
  * times a power of two: exact in 32 bits, the same for any order of summation.  NaN in q counts as 0.
- * max_seq_len bounds every row's length (a longer one is cut to it) and sizes the workspace, which need not be
- * cleared: drk_block_select_workspace_bytes, 16-byte aligned.  1 <= n_keep, n_sink + n_recent <= n_keep; at most 16
+ * max_seq_len bounds every row's length (a longer one is cut to it, as it is to the table_stride blocks of a table
+ * row) and sizes the workspace, which need not be cleared: drk_block_select_workspace_bytes, 16-byte aligned.  1 <= n_keep, n_sink + n_recent <= n_keep; at most 16
  * query heads per kv head; head_dim as for the bounds; io_dtype DRK_F16 / DRK_BF16.  Rows of length <= 0 get -1. */
 size_t drk_block_select_workspace_bytes(const drk_kv_layout *g, int T, int max_seq_len);
 int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, const void *q, int io_dtype,
@@ -556,8 +557,8 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
                      size_t workspace_bytes, void *stream);
 
 /* GQA attention of T query rows over the blocks listed for each (row, kv head): d_selected [T][num_kv_heads][n_keep]
- * logical blocks in any order; an entry that is negative, lies behind the row's last token, or has no page is passed
- * over, one that is listed twice counts twice.  Rows, lengths and tables as in drk_block_select; q / out
+ * logical blocks in any order; an entry that is negative, lies behind the row's last token or its table, or has no page is
+ * passed over, one that is listed twice counts twice.  Rows, lengths and tables as in drk_block_select; q / out
  * [T, num_q_heads, head_dim] of io_dtype; a row sees only its first seq_len tokens.  out = attention, or with a gate
  * attention * sigmoid(gate) (rows gate_stride elements apart, 16-byte aligned), rounded once; a row without a token,
  * or whose every score is -inf, is left as it was.  head_dim 128 or 256, block_size % 16 == 0, at most 16 query heads per kv head, every storage

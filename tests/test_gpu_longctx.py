@@ -429,6 +429,22 @@ def test_select_odd_queries(dev):
         assert np.array_equal(got[t], R.select(qf[t], codes[0], exps[0], tables[t], n * bs, bs, 7, 0, 0)), t
 
 
+@pytest.mark.parametrize("n", [6, 300, 2500])
+def test_select_never_reads_past_a_table_row(dev, n):
+    """Lengths beyond the table's blocks are cut to it, whichever kernels the size calls for."""
+    rng = np.random.default_rng(n)
+    D, QH, KVH, bs, io = 128, 8, 2, 4, cabi.F16
+    tables = np.stack([rng.permutation(n).astype(np.int32) for _ in range(3)])
+    g = cabi.layout(1, KVH, QH, D, bs, n, io)
+    codes, exps = R.bounds_buffers(1, n, KVH, D, rng)
+    q = U.normal_bits(rng, (3, QH, D), io)
+    lens = np.array([n * bs + 50, n * bs - 3, 2 ** 31 - 1], np.int32)
+    got = run_select(g, R.bounds_bytes(codes, exps), q, tables, n, lens, 0, 3, n * bs + 200, 5, 1, 2, io)
+    qf = U.from_bits(q, io).astype(np.float64)
+    for t in range(3):
+        assert np.array_equal(got[t], R.select(qf[t], codes[0], exps[0], tables[t], min(int(lens[t]), n * bs), bs, 5, 1, 2)), t
+
+
 # ---- attention --------------------------------------------------------------------------------
 def run_attend(p, q, tables, stride, lens, start, sel, io, layer=0, gate=None, gate_stride=0, scale=None):
     T, keep = q.shape[0], sel.shape[2]
@@ -511,6 +527,20 @@ def test_attend_branches(dev, dtype, geo, gated):
                   1 / math.sqrt(D), io, dgate.data_ptr() + 2 * D, 2 * D, U.p(ws), need, U.stream_ptr())
         U.sync()
         assert np.array_equal(U.host(out2, np.uint16, got.shape), got)
+
+
+def test_attend_passes_over_entries_behind_the_table(dev):
+    rng = np.random.default_rng(5)
+    D, QH, KVH, bs, n, io = 128, 8, 2, 16, 3, cabi.BF16
+    p = R.Pool(rng, 1, KVH, QH, D, bs, 4 * n, io)
+    tables = rng.permutation(4 * n).astype(np.int32).reshape(4, n)
+    lens = np.full(4, 100 * bs, np.int32)                                   # longer than the tables
+    sel = np.tile(np.array([0, 2, n, n + 1, 99, -1], np.int32), (4, KVH, 1))
+    sel[2] = [n, n + 7, 50, -1, 99, 98]                                     # nothing of it is in the table
+    q = U.normal_bits(rng, (4, QH, D), io)
+    got = run_attend(p, q, tables, n, lens, 0, sel, io)
+    inside = np.where(sel < n, sel, -1)
+    check_attend(p, got, q, tables, np.full(4, n * bs, np.int32), inside, io)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -56,6 +56,16 @@ def test_rope_refusals():
     assert code("drk_rope_table_fill_scaled", cabi.rope(64, True), P, 5, None) == cabi.ERR_UNSUPPORTED
 
 
+def test_rope_refuses_rows_that_two_threads_would_write():
+    ok = cabi.rope(64)
+    for rows in ([(P, 2 * P, 8, 1024, 128, 512, 128)],                         # tokens inside one another's heads
+                 [(P, 2 * P, 1, 128, 128, 0, 0)], [(P, 2 * P, 1, 128, 128, 120, 128)],
+                 [(P, 2 * P, 8, 128, 512, 128, 384)],                          # heads inside one another's tokens
+                 [(P, P, 8, 1024, 128, 1024, 128), (P, P, 8, 1024, 128, 1024, 128)],
+                 [(P, 2 * P, 8, 1024, 128, 1024, 128), (3 * P, 2 * P, 2, 256, 128, 256, 128)]):
+        assert rope_code(ok, rows=rows) == cabi.ERR_INVALID, rows
+
+
 def test_bounds_refusals_and_bytes():
     L = cabi.lib()
     for kw in (dict(), dict(D=512, dtype=cabi.INT8), dict(D=64, bs=7, KVH=3, QH=3)):

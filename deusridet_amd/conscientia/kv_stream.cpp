@@ -266,7 +266,7 @@ bool KvStream::set_sparse_decode(int min_tokens, int n_keep, int n_sink, int n_r
     const BlockPool& pool = cm_->block_pool();
     const int bs = pool.block_size(), nb = pool.max_blocks();
     if (min_tokens < 0 || n_keep < 0 || n_sink < 0 || n_recent < 0 || n_sink > n_keep || n_recent > n_keep - n_sink ||
-        !paged_sparse_attention_supported(bs) || (scorer_ && scorer_->d_new_scores()) || cm_->has_overflow_tier()) {
+        !paged_sparse_attention_supported(bs) || scorer_ || cm_->has_overflow_tier()) {
         LOG_ERROR("Conscientia", "KvStream: decode over selected blocks (keep %d, %d first, %d last) is not possible here", n_keep, n_sink,
                   n_recent);
         return false;

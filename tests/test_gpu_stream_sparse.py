@@ -179,3 +179,10 @@ def test_refusals(dev, tmp_path):
     scored = S.Session(1, scorer=True)
     assert not scored.ks.set_sparse_decode(0, 4, 1, 1)
     assert not host.KvStream().set_sparse_decode(0, 4, 1, 1)         # not initialised
+
+
+def test_a_scorer_that_is_not_ready_yet_is_refused_too(dev):
+    s = S.Session(1)
+    sc, ks = host.ImportanceScorer(), host.KvStream()
+    assert ks.init(s.cm, S.NPOS, sc, U.p(s.dtab), S.NPOS)
+    assert not ks.set_sparse_decode(0, 4, 1, 1)

@@ -673,6 +673,62 @@ def test_chunk_over_selected_blocks_through_the_host_functions(dev, dtype):
 
 
 # ---- together ---------------------------------------------------------------------------------
+@pytest.mark.parametrize("D,bs,dtype", [(128, 16, cabi.BF16), (256, 64, cabi.INT8)])
+def test_pages_and_bounds_beyond_32_bit_offsets(dev, D, bs, dtype):
+    """The last pages of a layer of more than 4 GiB, the second of the pool, and bounds behind 4 GiB of others: what comes
+    out is what the same pages give in a small pool, bit for bit."""
+    import torch
+    KVH, QH, io, T, keep = 4, 8, cabi.BF16, 3, 5
+    rng = np.random.default_rng(bs)
+    p = R.Pool(rng, 1, KVH, QH, D, bs, 40, dtype)
+    L = cabi.lib()
+    block = L.drk_kv_block_stride_bytes(C.byref(p.g))
+    NB = (5 << 30) // block
+    layers = -(-(9 << 29) // (NB * KVH * 2 * D)) + 1                        # so many that the last one's bounds lie beyond 4 GiB
+    small_in_big = cabi.layout(2, KVH, QH, D, bs, NB, dtype)
+    many = cabi.layout(layers, KVH, QH, D, bs, NB, dtype)
+    big = torch.empty(L.drk_kv_pool_bytes(C.byref(small_in_big)), dtype=torch.uint8, device="cuda")
+    at = big.numel() // 2 + (NB - 40) * block
+    assert at - big.numel() // 2 > 1 << 32
+    big[at:at + 40 * block].copy_(U.dev_bytes(p.raw))
+    tables = rng.permutation(40)[:36].astype(np.int32).reshape(T, 12)
+    lens = np.array([12 * bs - 3, 5 * bs + 1, 7 * bs], np.int32)
+    q = U.dev_bytes(U.normal_bits(rng, (T, QH, D), io))
+    dl = U.dev_i32(lens)
+
+    def run(g, pool, layer, bg, blayer, tab):
+        """bounds of `layer` of the pool into that layer of a buffer, then moved to layer `blayer` of the selection's layout"""
+        db = torch.zeros(L.drk_kv_bounds_bytes(C.byref(g)), dtype=torch.uint8, device="cuda")
+        dt = U.dev_i32(tab)
+        for t in range(T):
+            cabi.call("drk_kv_bounds_update", g, U.p(pool), dt.data_ptr() + 48 * t, 0, None, 0, int(lens[t]), layer, 1, U.p(db), U.stream_ptr())
+        if bg is not g:
+            n, n1 = NB * KVH * 2 * D, NB * KVH
+            wide = torch.empty(L.drk_kv_bounds_bytes(C.byref(bg)), dtype=torch.uint8, device="cuda")
+            wide[blayer * n:(blayer + 1) * n].copy_(db[layer * n:(layer + 1) * n])
+            wide[layers * n + blayer * n1:layers * n + (blayer + 1) * n1].copy_(db[2 * n + layer * n1:2 * n + (layer + 1) * n1])
+            db = wide
+        ids = U.dev_i32(tab.reshape(-1))
+        values = torch.empty(36 * KVH * 2 * D, dtype=torch.int16, device="cuda")
+        cabi.call("drk_kv_bounds_extract", bg, U.p(values), U.p(db), U.p(ids), 36, blayer, 1, U.stream_ptr())
+        sel = U.dev_i32(np.zeros((T, KVH, keep)))
+        ws = U.dev_zeros(max(L.drk_block_select_workspace_bytes(C.byref(bg), T, 12 * bs), L.drk_paged_sparse_workspace_bytes(C.byref(g), T, keep)))
+        cabi.call("drk_block_select", bg, U.p(db), blayer, U.p(q), io, U.p(dt), 12, U.p(dl), 0, T, 12 * bs, keep, 1, 1, U.p(sel), U.p(ws),
+                  ws.numel(), U.stream_ptr())
+        out = U.dev_zeros(T * QH * D * 2)
+        cabi.call("drk_paged_sparse_attention", g, U.p(q), U.p(pool), U.p(dt), 12, U.p(dl), 0, T, U.p(sel), keep, U.p(out), layer,
+                  1 / math.sqrt(D), io if dtype == cabi.INT8 else dtype, None, 0, U.p(ws), ws.numel(), U.stream_ptr())
+        U.sync()
+        return U.host(values, np.int16), U.host(sel, np.int32), U.host(out, np.uint16)
+
+    dp = U.dev_bytes(p.raw)
+    near = run(p.g, dp, 0, p.g, 0, tables)
+    far = run(small_in_big, big, 1, many, layers - 1, (tables + (NB - 40)).astype(np.int32))
+    for a, b in zip(near, far):
+        assert np.array_equal(a, b)
+    assert near[2].any()
+
+
 def test_a_decode_step_of_all_four_eager_and_captured(dev):
     """Rotation out of the Q | gate projection, append, bounds, selection, attention: three branches, three steps; then the
     same steps from a captured graph, with eager work between the replays."""

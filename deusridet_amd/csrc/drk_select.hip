@@ -203,11 +203,54 @@ __device__ __forceinline__ uint32_t sel_key_of(const SelArgs &A, uint32_t scored
     return none ? 0u : (forced ? kKeyForced : scored);
 }
 
+// The codes of 16 blocks on their way to a wave's operands.  An operand's neighbouring lanes hold neighbouring blocks, and lanes
+// 16 apart the same block's chunks: read like that, every lane is an access of its own (51 per load, 9.4 M of them for
+// 16 branches x 64k: the score kernel's time).  So the wave reads whole blocks, lane after lane, and exchanges the
+// chunks through LDS, chunk x of block c in place x ^ swap(c), which puts 16 neighbouring lanes on 16 different
+// 16-byte places of the 256 that the banks hold.  The wave's own region: no barrier.
+__device__ __forceinline__ int sel_swap(int D, int c) { return D == 64 ? c >> 1 : c; }
+// the entry (block * KVH + head) of block c of the group lies behind the table entry in lane base + c
+template <int D>
+__device__ __forceinline__ void sel_fetch(sel_i32x4 (&v)[D / 32], const uint8_t *bounds, const Lay &a, int h, int ahead, int base, int lane)
+{
+    constexpr int CH = D / 8;                                // 16-byte chunks of a block
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+        const int x = i * 64 + lane, blk = __shfl(ahead, base + x / CH);
+        const size_t entry = (size_t)((unsigned)blk < (unsigned)a.NB ? blk : 0) * a.KVH + h;   // block 0 is always mapped; its score is not used
+        v[i] = *(const sel_i32x4 *)(bounds + entry * (2 * D) + (x & (CH - 1)) * 16);
+    }
+}
+template <int D>
+__device__ __forceinline__ void sel_stage(sel_i32x4 *lds, const sel_i32x4 (&v)[D / 32], int lane)
+{
+    constexpr int CH = D / 8;
+#pragma unroll
+    for (int i = 0; i < D / 32; i++) {
+        const int x = i * 64 + lane, c = x / CH;
+        lds[c * CH + ((x & (CH - 1)) ^ sel_swap(D, c))] = v[i];
+    }
+}
+template <int D>
+__device__ __forceinline__ sel_i32x4 sel_operand(const sel_i32x4 *lds, int k, int g, int c)
+{
+    return lds[c * (D / 8) + ((k * 4 + g) ^ sel_swap(D, c))];
+}
+// what other lanes of the wave wrote to LDS before is there, what they read has been read
+__device__ __forceinline__ void sel_wave_order()
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#endif
+}
+
 // One set of 16 heads per wave: a branch's row (R = 1), or R = 16 / P rows of one table.
 template <int D>
 __global__ __launch_bounds__(256) void score_kernel(Lay a, SelArgs A)
 {
     constexpr int KS = D / 32;
+    __shared__ sel_i32x4 codes[4][16 * D / 8];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int h = blockIdx.x, GQ = a.QH / a.KVH;           // kv heads vary fastest: a block's codes of all heads lie together
     const int row0 = blockIdx.z * A.R;
@@ -227,25 +270,19 @@ __global__ __launch_bounds__(256) void score_kernel(Lay a, SelArgs A)
 #pragma unroll
     for (int j = 0; j < 4; j++) qm[j] = sel_pow2(__shfl(eq, 4 * g + j));
 
-    uint4 bv[KS];
+    sel_i32x4 bv[KS];
     int eb = 0;
     auto fetch = [&](int i) {                                                   // group first + i; ahead holds its entries
+        sel_fetch<D>(bv, A.bounds, a, h, ahead, (i & 3) * 16, lane);
         const int blk = __shfl(ahead, (i & 3) * 16 + c);
-        const bool hole = blk < 0 || blk >= a.NB;
-        const size_t entry = (size_t)(hole ? 0 : blk) * a.KVH + h;              // block 0 is always mapped; its score is not used
-        const uint8_t *cp = A.bounds + entry * (2 * D) + g * 16;
-#pragma unroll
-        for (int k = 0; k < KS; k++) bv[k] = *(const uint4 *)(cp + k * 64);
-        eb = hole ? kNoBlock : (int)(int8_t)A.exps[entry];
+        eb = (unsigned)blk < (unsigned)a.NB ? (int)(int8_t)A.exps[(size_t)blk * a.KVH + h] : kNoBlock;
     };
     fetch(0);
     const int n = min(A.groups_per_wave, (nbmax + 15) / 16 - first);
     for (int i = 0; i < n; i++) {
-        sel_i32x4 acc = {0, 0, 0, 0};
-#if defined(__HIP_DEVICE_COMPILE__)
-#pragma unroll
-        for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[k], __builtin_bit_cast(sel_i32x4, bv[k]), acc, 0, 0, 0);
-#endif
+        sel_wave_order();
+        sel_stage<D>(codes[w], bv, lane);
+        sel_wave_order();
         const int e = eb;
         if (i + 1 < n) {
             if (((i + 1) & 3) == 0) {
@@ -254,6 +291,11 @@ __global__ __launch_bounds__(256) void score_kernel(Lay a, SelArgs A)
             }
             fetch(i + 1);
         }
+        sel_i32x4 acc = {0, 0, 0, 0};
+#if defined(__HIP_DEVICE_COMPILE__)
+#pragma unroll
+        for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[k], sel_operand<D>(codes[w], k, g, c), acc, 0, 0, 0);
+#endif
         const uint32_t x = sel_row_key(acc, qm, A.P, e == kNoBlock ? 0.0f : sel_pow2(e));
         const int b = (first + i) * 16 + c;
         if ((A.R > 1 ? ((4 * g) & (A.P - 1)) == 0 : g == 0) && row < A.T && (unsigned)b < A.key_stride)

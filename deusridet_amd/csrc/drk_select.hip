@@ -26,9 +26,9 @@ namespace drk {
 
 constexpr uint32_t kKeyForced = 0xffffffffu;
 // Contexts of few blocks are scored and selected by one workgroup per (row, kv head) in one launch: a second launch costs
-// about 3 us, one workgroup reads about 100 GB/s.  Branches of 8 kv heads x 128: 94 blocks 7.0 us; 500 blocks 10.6 where
-// the two kernels take 9; 1000 blocks 14.8.
-constexpr size_t kSelFusedBytes = 80 << 10;    // codes of the context per kv head, with few rows
+// about 3 us, one workgroup reads some 60 GB/s.  A branch of 8 kv heads x 128: 250 blocks 6.9 us; 500 blocks 8.2 where the
+// two kernels take 10.1; 750 blocks 9.5 and 10.1; 1000 blocks 10.6 and 9.7.
+constexpr size_t kSelFusedBytes = 200 << 10;   // codes of the context per kv head, with few rows
 constexpr int kSelFusedRows = 256;             // (row, kv head) pairs that keep every CU busy by themselves
 constexpr int kSelFused = 1024;                // blocks, the most that kernel takes
 constexpr int kSelShort = 128;                 // blocks up to which chunks take it too, and fewer threads do
@@ -674,6 +674,7 @@ __global__ __launch_bounds__(THREADS) void select_kernel(Lay a, SelArgs A)
     static_assert(GPW * 16 * W == BLOCKS && GPW % G == 0, "whole rounds of groups");
     __shared__ TopkLds<THREADS> S;
     __shared__ uint32_t key_lds[BLOCKS];
+    __shared__ sel_i32x4 codes[W][16 * D / 8];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int t = blockIdx.x / a.KVH, h = blockIdx.x - t * a.KVH, GQ = a.QH / a.KVH;
     const int32_t *tab = A.tables + (size_t)t * A.table_stride;
@@ -686,7 +687,7 @@ __global__ __launch_bounds__(THREADS) void select_kernel(Lay a, SelArgs A)
     for (int j = 0; j < 4; j++) qm[j] = sel_pow2(__shfl(eq, 4 * g + j));
     for (int g0 = w; g0 < groups; g0 += G * W) {
         int blk[G], e[G];
-        uint4 bv[G][KS];
+        sel_i32x4 bv[G][KS];
 #pragma unroll
         for (int i = 0; i < G; i++) {
             const int b = (g0 + i * W) * 16 + c;
@@ -695,21 +696,20 @@ __global__ __launch_bounds__(THREADS) void select_kernel(Lay a, SelArgs A)
 #pragma unroll
         for (int i = 0; i < G; i++) {
             if (g0 + i * W >= groups) continue;                          // the same for the whole wave
-            const bool hole = blk[i] < 0 || blk[i] >= a.NB;
-            const size_t entry = (size_t)(hole ? 0 : blk[i]) * a.KVH + h;      // block 0 is always mapped; its score is not used
-            const uint8_t *cp = A.bounds + entry * (2 * D) + g * 16;
-#pragma unroll
-            for (int k = 0; k < KS; k++) bv[i][k] = *(const uint4 *)(cp + k * 64);
-            e[i] = hole ? kNoBlock : (int)(int8_t)A.exps[entry];
+            sel_fetch<D>(bv[i], A.bounds, a, h, blk[i], 0, lane);
+            e[i] = (unsigned)blk[i] < (unsigned)a.NB ? (int)(int8_t)A.exps[(size_t)blk[i] * a.KVH + h] : kNoBlock;
         }
 #pragma unroll
         for (int i = 0; i < G; i++) {
             if (g0 + i * W >= groups) continue;
             const int b = (g0 + i * W) * 16 + c;
+            sel_wave_order();
+            sel_stage<D>(codes[w], bv[i], lane);
+            sel_wave_order();
             sel_i32x4 acc = {0, 0, 0, 0};
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
-            for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[k], __builtin_bit_cast(sel_i32x4, bv[i][k]), acc, 0, 0, 0);
+            for (int k = 0; k < KS; k++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[k], sel_operand<D>(codes[w], k, g, c), acc, 0, 0, 0);
 #endif
             const uint32_t x = sel_row_key(acc, qm, A.P, e[i] == kNoBlock ? 0.0f : sel_pow2(e[i]));
             if (g == 0) key_lds[b] = sel_key_of(A, x, b, nb, e[i]);

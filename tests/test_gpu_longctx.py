@@ -429,6 +429,23 @@ def test_select_odd_queries(dev):
         assert np.array_equal(got[t], R.select(qf[t], codes[0], exps[0], tables[t], n * bs, bs, 7, 0, 0)), t
 
 
+@pytest.mark.parametrize("n", [1500, 2100, 4200, 8300])
+def test_select_many_rows_of_many_blocks(dev, n):
+    """More (row, kv head) pairs than workgroups are wanted: the selection's other shapes, with ties among coarse bounds."""
+    rng = np.random.default_rng(n)
+    D, KVH, T, io = 64, 8, 66, cabi.BF16
+    g = cabi.layout(1, KVH, KVH, D, 1, n, io)
+    codes, exps = R.bounds_buffers(1, n, KVH, D, rng)
+    codes[:, n // 2:] = np.sort(np.sign(codes[:, n // 2:]), 3)              # -1, 0, 1, low <= high: many equal scores
+    exps[:, n // 2:] = 3
+    q = U.normal_bits(rng, (T, KVH, D), io)
+    table = rng.permutation(n).astype(np.int32)
+    got = run_select(g, R.bounds_bytes(codes, exps), q, table, 0, None, n - T, T, n, 40, 1, 3, io)
+    qf = U.from_bits(q, io).astype(np.float64)
+    for t in (0, 1, 30, 31, 64, 65):
+        assert np.array_equal(got[t], R.select(qf[t], codes[0], exps[0], table, n - T + t + 1, 1, 40, 1, 3)), t
+
+
 @pytest.mark.parametrize("n", [6, 300, 2500])
 def test_select_never_reads_past_a_table_row(dev, n):
     """Lengths beyond the table's blocks are cut to it, whichever kernels the size calls for."""

@@ -10,6 +10,11 @@
 //   O[head][dim]  += P[heads x 16] V     D/16 x v_mfma_f32_16x16x16
 // with the query heads of the group as the 16-wide operand.  The waves' states meet at the end; a row
 // that was cut leaves (o, m, l) per piece for sparse_merge_kernel, otherwise it is written at once.
+//
+// Bound by HBM for branches: 64 x 256 blocks of 16 tokens x 8 heads x 128 (1.08 GB bf16) 169 us, 6.4 TB/s (183 with other pages
+// every time: translations); 16 x 128 blocks int8 (69 MB) 17 us, of which the walk is 10, the rest launch, list, table,
+// first pages and the end, + 4 for the merge; 1 x 64 blocks 6 + 3 us, all of it latency.  Rows of a chunk meet in the L2
+// instead: 512 x 64 blocks (2.1 GB from 134 MB of pages) 124 us, 17 TB/s, two thirds of the lines from the L2.
 #include "drk_stream_tile.hpp"
 
 namespace drk {
@@ -450,7 +455,7 @@ static int sparse_pieces(const Lay &a, int T, int n_keep, int *groups_per_piece)
 }
 
 // Waves per row: as few as still give the chip the waves it holds (16 per CU at head_dim 128, 8 at 256) and leave
-// room in LDS for that many.
+// room in LDS for that many: fewer waves per row, fewer states to fold (512 rows x 64 blocks: one wave 128 us, eight 183).
 static int sparse_waves_per_row(const Lay &a, int T, int groups_per_piece)
 {
     const size_t rows = (size_t)T * a.KVH, waves = a.D == 128 ? 4096 : 2048;
@@ -535,7 +540,9 @@ int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void
     A.row_bytes = a.row_bytes;
     A.scale_log2e = scale * kSLog2e;
     hipStream_t st = (hipStream_t)stream;
-    const bool shared = table_stride == 0 && T > 1;           // rows over one table meet in the same pages: keep them cached
+    // rows over one table meet in the same pages: keep them cached (512 rows 128 us, non-temporal 244); branches do not
+    // (64 x 256 blocks non-temporal 191, cached 210)
+    const bool shared = table_stride == 0 && T > 1;
     const int wpr = A.pieces > 1 ? 8 : sparse_waves_per_row(a, T, A.groups_per_piece);
     const int per_wg = kSpWaves / wpr;                        // rows of a workgroup
     const dim3 grid((unsigned)(((size_t)T + per_wg - 1) / per_wg * A.pieces * a.KVH));

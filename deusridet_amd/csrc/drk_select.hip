@@ -16,8 +16,8 @@
 //   reads.  Bound by the bytes of the bounds: 16 branches x up to 64k (101 MB) 20 us, 5.1 TB/s and about 5 us of launch, length,
 //   table and first codes; one branch x 32k 4 us.
 //   score_tile_kernel: rows of one table; 8 waves x 2 sets of heads meet the same blocks, which pass through LDS.  512 rows x
-//   24 heads x 1970 blocks of head_dim 256: 32 us, 1.55 POP/s of the GQ heads (2.1 with the rows that fill up an operand of
-//   8): per 32 blocks and wave 32 products (512 clocks), 16 LDS reads and 123 vector instructions (about as long each), which
+//   24 heads x 1970 blocks of head_dim 256: 32 us, 0.77 POP/s (1.03 with the rows that fill up an operand: 8 for 6 heads):
+//   per 32 blocks and wave 32 products (512 clocks), 16 LDS reads and 123 vector instructions (about as long each), which
 //   two waves per SIMD overlap by half; another 5 us are the queries' conversion.
 // topk_kernel: one workgroup per (row, kv head) finds the n_keep-th key: a histogram over the range the keys
 // really span leaves a handful in one bin, which every wave then settles by itself with ballots; the chosen

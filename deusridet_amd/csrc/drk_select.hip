@@ -16,7 +16,7 @@
 //   reads.  Bound by the bytes of the bounds: 16 branches x up to 64k (101 MB) 20 us, 5.1 TB/s and about 5 us of launch, length,
 //   table and first codes; one branch x 32k 4 us.
 //   score_tile_kernel: rows of one table; 8 waves x 2 sets of heads meet the same blocks, which pass through LDS.  512 rows x
-//   24 heads x 1970 blocks of head_dim 256: 32 us, 0.77 POP/s (1.03 with the rows that fill up an operand: 8 for 6 heads):
+//   24 heads x 1970 blocks of head_dim 256: 29 us, 0.84 POP/s (1.13 with the rows that fill up an operand: 8 for 6 heads):
 //   per 32 blocks and wave 32 products (512 clocks), 16 LDS reads and 123 vector instructions (about as long each), which
 //   two waves per SIMD overlap by half; another 5 us are the queries' conversion.
 // topk_kernel: one workgroup per (row, kv head) finds the n_keep-th key: a histogram over the range the keys
@@ -26,6 +26,8 @@
 #include "drk_common.hpp"
 #include "drk_codec.hpp"
 #include "drk_bounds.hpp"
+
+#include <type_traits>
 
 namespace drk {
 
@@ -333,39 +335,39 @@ __global__ __launch_bounds__(512) void score_tile_kernel(Lay a, SelArgs A)
     if (first * 16 >= nbmax) return;
     const int n = (min(A.groups_per_wave, (nbmax + 15) / 16 - first) + G - 1) / G;         // steps
 
-    // thread (r0, ch) brings chunk ch of blocks r0, r0 + 512 / CH, .. of a step; ahead: their table entries
+    // Thread (r0, ch) brings chunk ch of blocks r0, r0 + 512 / CH, .. of a step, requested two steps ahead, by table entries
+    // requested two steps before that.  Even and odd steps have registers of their own and every request is made by every thread
+    // (clamped instead of skipped): loads and stores are counted in order, so that a wait for a step's codes lets what
+    // was requested after them travel on -- unless the compiler has to reckon with requests that were not made.
     const int r0 = (int)threadIdx.x / CH, ch = (int)threadIdx.x - r0 * CH;
-    uint4 st[2][PER];
-    int es[2][PER], ahead[PER];
-    auto page = [&](int i) {
+    sel_i32x4 st[2][PER];
+    int es[2][PER], ahead[2][PER];
+    bool hole[2][PER];
+    auto page = [&](int q, int i) {
+#pragma unroll
+        for (int u = 0; u < PER; u++) ahead[q][u] = A.tables[min((first + i * G) * 16 + r0 + u * (512 / CH), nbmax - 1)];
+    };
+    auto fetch = [&](int q, int i) {
 #pragma unroll
         for (int u = 0; u < PER; u++) {
-            const int r = r0 + u * (512 / CH), lb = (first + i * G) * 16 + r;
-            ahead[u] = r < 16 * G && lb < nbmax ? A.tables[lb] : -1;
+            hole[q][u] = (unsigned)ahead[q][u] >= (unsigned)a.NB || (first + i * G) * 16 + r0 + u * (512 / CH) >= nbmax;
+            const size_t entry = (size_t)(hole[q][u] ? 0 : ahead[q][u]) * a.KVH + h;     // block 0 is always mapped
+            st[q][u] = *(const sel_i32x4 *)(A.bounds + entry * (2 * D) + ch * 16);
+            es[q][u] = (int)(int8_t)A.exps[entry];
         }
     };
-    auto fetch = [&](int s) {
-#pragma unroll
-        for (int u = 0; u < PER; u++) {
-            const bool hole = ahead[u] < 0 || ahead[u] >= a.NB;
-            const size_t entry = (size_t)(hole ? 0 : ahead[u]) * a.KVH + h;     // block 0 is always mapped
-            if (r0 + u * (512 / CH) < 16 * G) st[s][u] = *(const uint4 *)(A.bounds + entry * (2 * D) + ch * 16);
-            es[s][u] = hole ? kNoBlock : (ch == 0 ? (int)(int8_t)A.exps[entry] : 0);
-        }
-    };
-    auto stage = [&](int buf) {                               // the older of the two sets in flight
+    auto stage = [&](int q) {
 #pragma unroll
         for (int u = 0; u < PER; u++) {
             const int r = r0 + u * (512 / CH);
-            if (r < 16 * G) *(uint4 *)(b_lds[buf] + r * PITCH + ch * 16) = st[0][u];
-            if (r < 16 * G && ch == 0) e_lds[buf][r] = es[0][u];
-            st[0][u] = st[1][u];
-            es[0][u] = es[1][u];
+            if (r < 16 * G) *(sel_i32x4 *)(b_lds[q] + r * PITCH + ch * 16) = st[q][u];
+            if (r < 16 * G && ch == 0) e_lds[q][r] = hole[q][u] ? kNoBlock : es[q][u];
         }
     };
-    page(0);
-    fetch(0);
-    page(1);
+    page(0, 0);
+    page(1, 1);
+    fetch(0, 0);
+    page(0, 2);
     sel_i32x4 qa[SETS][KS];
     float qm[SETS][4];
     int nbr[SETS];
@@ -388,14 +390,20 @@ __global__ __launch_bounds__(512) void score_tile_kernel(Lay a, SelArgs A)
 #pragma unroll
     for (int off = 16; off < 64; off <<= 1) nbmin = min(nbmin, __shfl_xor(nbmin, off));
     const int scored_end = __builtin_amdgcn_readfirstlane(nbmin) - A.recent;    // from the first blocks to here every row only scores
-    fetch(1);
-    page(2);
+    // a key that is not to be stored gets an offset beyond the buffer, which the store drops: see above, no store is skipped
+    const __amdgpu_buffer_rsrc_t krsrc = __builtin_amdgcn_make_buffer_rsrc(kbase, 0, (int)(64u * (unsigned)a.KVH * A.key_stride * 4), 0x00027000);
+    fetch(1, 1);
+    page(1, 3);
     stage(0);
     __syncthreads();
-    for (int i = 0; i < n; i++) {
-        fetch(1);
-        page(i + 3);
-        const uint8_t *buf = b_lds[i & 1];
+    auto step = [&](auto parity, int i) {
+        constexpr int q = decltype(parity)::value;
+        fetch(q, i + 2);
+        page(q, i + 4);
+#if defined(__HIP_DEVICE_COMPILE__)
+        __builtin_amdgcn_sched_barrier(0);
+#endif
+        const uint8_t *buf = b_lds[q];
         uint4 bv[G][KS];
 #pragma unroll
         for (int x = 0; x < G; x++)
@@ -416,7 +424,7 @@ __global__ __launch_bounds__(512) void score_tile_kernel(Lay a, SelArgs A)
                 }
 #pragma unroll
         for (int x = 0; x < G; x++) {
-            const int e = e_lds[i & 1][x * 16 + c], b0 = (first + i * G + x) * 16, b = b0 + c;
+            const int e = e_lds[q][x * 16 + c], b0 = (first + i * G + x) * 16, b = b0 + c;
             const bool hole = e == kNoBlock, inner = b0 >= A.sink && b0 + 16 <= scored_end;
             const float bm = hole ? 0.0f : sel_pow2(e);
             uint32_t key[SETS];
@@ -431,10 +439,17 @@ __global__ __launch_bounds__(512) void score_tile_kernel(Lay a, SelArgs A)
             }
 #pragma unroll
             for (int s = 0; s < SETS; s++)
-                if (on[s] & ((unsigned)b < A.key_stride)) kbase[ko[s] + (unsigned)b] = key[s];
+                __builtin_amdgcn_raw_buffer_store_b32(key[s], krsrc, (on[s] & ((unsigned)b < A.key_stride)) ? (int)((ko[s] + (unsigned)b) * 4) : -1, 0, 0);
         }
-        stage((i + 1) & 1);
+#if defined(__HIP_DEVICE_COMPILE__)
+        __builtin_amdgcn_sched_barrier(0);
+#endif
+        stage(1 - q);
         __syncthreads();
+    };
+    for (int i = 0; i < n; i += 2) {                         // a step too many meets holes
+        step(std::integral_constant<int, 0>(), i);
+        step(std::integral_constant<int, 1>(), i + 1);
     }
 }
 
@@ -743,9 +758,9 @@ static unsigned sel_key_stride(const Lay &a, int max_seq_len)
 static int sel_tile_groups(const Lay &a, unsigned groups, unsigned rows)
 {
     const unsigned least = a.D <= 128 ? (groups + 63) / 64 : 1;
-    unsigned best = 0xffffffffu, take = 2;
+    unsigned best = 0xffffffffu, take = 4;
     for (unsigned parts = least; parts == least || (parts <= groups && rows * parts <= 4 * kSelTileWgs); parts++) {
-        const unsigned g = ((groups + parts - 1) / parts + 1) & ~1u;
+        const unsigned g = ((groups + parts - 1) / parts + 3) & ~3u;
         const unsigned per_cu = (rows * ((groups + g - 1) / g) + kSelTileWgs - 1) / kSelTileWgs;
         const unsigned cost = (a.D <= 128 && per_cu > 1 ? 4 : 5) * per_cu * (g + kSelTileStart);
         if (cost < best) { best = cost; take = g; }
@@ -817,8 +832,8 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
     A.P = 4;
     while (A.P < a.QH / a.KVH) A.P *= 2;
     A.R = table_stride == 0 && T > 1 ? 16 / A.P : 1;
-    // more than four sets of rows over one table; its keys are counted in 32 bits over the 64 rows of a workgroup
-    const bool tile = table_stride == 0 && a.D <= 256 && T > 4 * A.R && (size_t)a.KVH * A.key_stride <= (1u << 26);
+    // more than four sets of rows over one table; a workgroup stores the keys of its 64 rows at 32-bit byte offsets
+    const bool tile = table_stride == 0 && a.D <= 256 && T > 4 * A.R && (size_t)a.KVH * A.key_stride <= (1u << 22);
     const int n = (int)(((size_t)max_seq_len + a.bs - 1) / a.bs);
     hipStream_t st = (hipStream_t)stream;
     if (n <= kSelShort || (n <= kSelFused && a.D <= 256 && !tile &&

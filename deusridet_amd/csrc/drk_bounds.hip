@@ -76,7 +76,7 @@ __device__ __forceinline__ BoundsUnit bounds_unit(const Lay &a, const BoundsArgs
         pos = A.d_pos[bi];
         lb = pos < 0 ? -1 : (int)dv((unsigned)pos, A.bs_div);
         tab += (size_t)bi * A.table_stride;
-        if (lb >= A.table_stride) lb = -1;
+        if (A.table_stride > 0 && lb >= A.table_stride) lb = -1;       // stride 0: one table for all, as long as its positions need
     } else {
         lb = A.first_block + (int)bi;
         pos = A.pos_start + A.n - 1;

@@ -525,8 +525,9 @@ int drk_rope_apply(const drk_rope *r, const double *d_freqs, const drk_rope_rows
  * head_dim is a power of two in [64, 512], any storage type, any block size. */
 size_t drk_kv_bounds_bytes(const drk_kv_layout *g);
 /* Recomputes, from the pages, the bounds of the blocks that received tokens; layers layer .. layer + layer_count - 1.
- * d_pos != NULL: one token for each of n branches, at d_pos[i] of table row i -- the block of d_pos[i] is covered up to
- * d_pos[i] (a negative position or a missing page is skipped).  NULL: tokens [pos_start, pos_start + n) of one table --
+ * d_pos != NULL: one token for each of n branches, at d_pos[i] of table row i * table_stride (0: one table for all, which
+ * every position lies in) -- the block of d_pos[i] is covered up to d_pos[i] (a negative position, one behind the
+ * table_stride blocks of its row, or a missing page is skipped).  NULL: tokens [pos_start, pos_start + n) of one table --
  * their blocks, up to pos_start + n - 1.  Tokens before pos_start in the first block count: the block is recomputed,
  * not added to, so copies made on write, reused pages and rewritten positions need nothing special.  Two branches at
  * different positions of one physical block, which the append does not allow either, leave its bounds undefined. */

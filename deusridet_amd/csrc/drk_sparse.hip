@@ -38,6 +38,26 @@ struct SparseArgs {
     float scale_log2e;
 };
 
+// The second product takes its weights in the 16-bit type its values come in (8-bit pages: fp16), rounded to nearest: a
+// 32-bit product would cost eight times the matrix instructions.  bf16 has fp32's range.  fp16 ends at 2^-24, and a wave may walk
+// 8192 tokens whose small weights count together: the largest weight is taken as 2^14 instead of 1, so that only what
+// is 2^39 below it vanishes.  With int8 pages the weight is p times the token's V scale, and all V scales may be 2^-14
+// or less: there the reference follows the largest p * scale, so that the product's weights fill the same range
+// whatever the scales are (p itself and its sum are in 32 bits).  Following p alone, a token 8 nats ahead of 2048 others with
+// scales of 2^-16 took their share of the output to nought; the time is the same (16 x 128 blocks int8 21.1 us).
+template <int DOT> constexpr float kSpHeadroom = DOT == DRK_BF16 ? 0.0f : 14.0f;
+
+// log2 of a V scale's magnitude, kept finite: nought (whose token only counts in the sum), infinity and NaN must not
+// become the reference
+__device__ __forceinline__ float sparse_log2_scale(float vs)
+{
+#if defined(__HIP_DEVICE_COMPILE__)
+    return fminf(fmaxf(__builtin_amdgcn_logf(fabsf(vs)), -24.0f), 16.0f);
+#else
+    return vs;
+#endif
+}
+
 // what a workgroup keeps in LDS beside the staged keys: the rows' query heads and group descriptors
 struct SparseLds {
     unsigned q, desc, total;             // bytes per row of queries / of descriptors (offsets, scale offsets, counts), all
@@ -198,13 +218,7 @@ __global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel
         const int lim = __builtin_amdgcn_readfirstlane((int)gcnt[i]);
         const bool more = i + W < n;
         stage_k<DT, D>(klds, kreg, lane);
-        float ks[4] = {1.0f, 1.0f, 1.0f, 1.0f}, vs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
-        if (DT == DRK_INT8) {
-            ks[0] = f16_bits_to_f((uint16_t)(ksr.x & 0xffffu)); ks[1] = f16_bits_to_f((uint16_t)(ksr.x >> 16));
-            ks[2] = f16_bits_to_f((uint16_t)(ksr.y & 0xffffu)); ks[3] = f16_bits_to_f((uint16_t)(ksr.y >> 16));
-            vs[0] = f16_bits_to_f((uint16_t)(vsr.x & 0xffffu)); vs[1] = f16_bits_to_f((uint16_t)(vsr.x >> 16));
-            vs[2] = f16_bits_to_f((uint16_t)(vsr.y & 0xffffu)); vs[3] = f16_bits_to_f((uint16_t)(vsr.y >> 16));
-        }
+        [[maybe_unused]] const uint2 ksc = ksr, vsc = vsr;     // packed until the softmax: registers
         uint32_t next = 0;
         if (more) {
             next = goff[i + W];
@@ -224,26 +238,31 @@ __global__ __launch_bounds__(kSpWaves * 64, D == 128 ? 4 : 2) void sparse_kernel
 #pragma unroll
             for (int kk = 0; kk < 4; kk++) sacc = w_mfma_qk<DOT>(ka[kk], qa[kk], sacc);
         }
-        // softmax of head c over tokens 4g..4g+3 (+ the other three lane groups)
+        // softmax of head c over tokens 4g..4g+3 (+ the other three lane groups): weights are 2^(sc - m_ref), m_ref the largest
+        // `top` so far less kSpHeadroom
         const int t0 = g * 4;
-        float sc[4], p[4];
+        float sc[4], top[4], p[4], vs[4] = {1.0f, 1.0f, 1.0f, 1.0f};
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             float x = sacc[j];
-            if (DT == DRK_INT8) x = (x - qbias) * ks[j];
+            if (DT == DRK_INT8) {
+                x = (x - qbias) * f16_bits_to_f((uint16_t)((j < 2 ? ksc.x : ksc.y) >> (16 * (j & 1)) & 0xffffu));
+                vs[j] = f16_bits_to_f((uint16_t)((j < 2 ? vsc.x : vsc.y) >> (16 * (j & 1)) & 0xffffu));
+            }
             x *= A.scale_log2e;
             sc[j] = t0 + j < lim ? x : -INFINITY;
+            top[j] = DT == DRK_INT8 ? sc[j] + sparse_log2_scale(vs[j]) : sc[j];
         }
-        float mloc = fmaxf(fmaxf(sc[0], sc[1]), fmaxf(sc[2], sc[3]));
+        float mloc = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         mloc = fmaxf(mloc, __shfl_xor(mloc, 16));
         mloc = fmaxf(mloc, __shfl_xor(mloc, 32));
         const float m_new = fmaxf(m_run, mloc), m_use = m_new == -INFINITY ? 0.0f : m_new;
-        const float alpha = s_exp2(m_run - m_use);
+        const float alpha = s_exp2(m_run - m_use), m_ref = m_use - kSpHeadroom<DOT>;
         m_run = m_new;
         float pw[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            p[j] = s_exp2(sc[j] - m_use);
+            p[j] = s_exp2(sc[j] - m_ref);
             pw[j] = DT == DRK_INT8 ? (t0 + j < lim ? p[j] * vs[j] : 0.0f) : p[j];
         }
         uint2 pa;                                             // P[head c][tokens 4g..4g+3] for the second product

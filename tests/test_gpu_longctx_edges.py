@@ -37,3 +37,95 @@ def test_bounds_of_branches_over_one_table(dev, dtype, bs):
                 G.check_block(p, codes, exps, layer, blk, written[blk])
             else:
                 assert (codes[layer, blk] == 0x55).all() and (exps[layer, blk] == 0x55).all()
+
+
+# ---- attention --------------------------------------------------------------------------------
+class SinkPages:
+    """Pages of one kv head in which the first token's key leads every other score by about `lead`, with a value of the
+    other sign: k, v float64 [NB, bs, D] of the stored numbers, vs [NB, bs] the V scales (int8), raw bytes."""
+
+    def __init__(self, rng, dtype, lead, vmag, NB=9, bs=256, D=128, QH=4):
+        self.dtype, self.NB, self.bs, self.D, self.QH = dtype, NB, bs, D, QH
+        self.io = dtype if dtype in (cabi.F16, cabi.BF16) else cabi.F16
+        base = rng.standard_normal(D)
+        self.q = U.to_bits((base * (1 - 0.02 * np.arange(QH)[:, None])).astype(np.float32), self.io)
+        k = rng.standard_normal((NB, bs, D)) * 0.05
+        k[0, 0] = base * lead * math.sqrt(D) / (base ** 2).sum()
+        if vmag == "mixed":                                    # scales over 2^20 within one list
+            vmag = 2.0 ** rng.uniform(-20, 0, (NB, bs, 1)) * 127
+            vmag[0, 0] = 2.0 ** -10 * 127
+        v = (0.5 + 0.5 * rng.random((NB, bs, D))) * vmag
+        v[0, 0] *= -1
+        self.vs = np.ones((NB, bs))
+        kv = np.stack([k, v], 1)                               # [NB, 2, bs, D]
+        if dtype in (cabi.F16, cabi.BF16):
+            bits = U.to_bits(kv.astype(np.float32), dtype)
+            kv, raw = U.from_bits(bits, dtype).astype(np.float64), bits.view(np.uint8)
+        elif dtype == cabi.INT8:
+            sc = (np.abs(kv).max(3) / 127).astype(np.float16)
+            scale = sc.astype(np.float64)
+            codes = np.clip(np.rint(kv / scale[..., None]), -127, 127).astype(np.int8)
+            kv, self.vs = codes * scale[..., None], scale[:, 1]
+            raw = np.concatenate([codes.view(np.uint8).reshape(NB, -1), sc.view(np.uint8).reshape(NB, -1)], 1)
+        else:
+            import torch
+            t = torch.from_numpy(kv.astype(np.float32)).to(torch.float8_e4m3fn)
+            kv, raw = t.double().numpy(), t.view(torch.uint8).numpy()
+        self.k, self.v, self.raw = kv[:, 0], kv[:, 1], np.ascontiguousarray(raw)
+        self.g = cabi.layout(1, 1, QH, D, bs, NB, dtype)
+
+    def want(self, sel, chain):
+        """Every listed token counted as often as its block is listed -> (out [QH, D], bound on what a kernel may be off by
+        before its last rounding): the weights' rounding to 16 bits, u (A + |out|) as in longctx_ref.attend; what a weight
+        below fp16's normal range loses, 2^-25 where the largest is 2^14; the scores' fp32 sums (int8: twenty times, as
+        there) and 2^-20 of the exponential, twice; `chain` dependent fp32 additions of the output."""
+        cnt = np.bincount(sel, minlength=self.NB).astype(np.float64)[:, None]
+        scale = 1 / math.sqrt(self.D)
+        out, tol = np.zeros((self.QH, self.D)), np.zeros((self.QH, self.D))
+        u = R.HALF_STEP[cabi.BF16 if self.dtype == cabi.BF16 else cabi.F16]
+        for i, q in enumerate(U.from_bits(self.q, self.io).astype(np.float64)):
+            s = self.k @ q * scale
+            p = cnt * np.exp(s - s[cnt[:, 0] > 0].max())
+            L = p.sum()
+            mean = lambda x: np.tensordot(p, x, 2) / L
+            o, A = mean(self.v), mean(np.abs(self.v))
+            one = np.exp(s - s[cnt[:, 0] > 0].max())
+            ds = (self.D + 8) * 2.0 ** -24 * (np.abs(self.k) @ np.abs(q))[cnt[:, 0] > 0].max() * scale
+            if self.dtype == cabi.INT8:
+                ds *= 20
+                wide = mean(self.vs)[None] * 1279
+                lost = (one * self.vs)[cnt[:, 0] > 0].max() * 127
+            else:
+                wide, lost = A, np.abs(self.v).max() + np.abs(o)
+            tail = 0.0 if self.dtype == cabi.BF16 else 1.01 * 2.0 ** -39 * cnt.sum() * self.bs * lost / L
+            out[i], tol[i] = o, u * (A + np.abs(o)) + tail + 2 * (ds + 2.0 ** -20) * A + chain * 2.0 ** -24 * wide
+        return out, tol
+
+
+@pytest.mark.parametrize("dtype,vmag,lead,keep,T", [
+    (cabi.INT8, 0.01, 8, 16, 1), (cabi.INT8, 0.002, 8, 16, 1), (cabi.INT8, 0.01, 8, 16, 1100),
+    (cabi.INT8, 0.002, 8, 16, 1100), (cabi.INT8, 30.0, 8, 16, 1),
+    (cabi.INT8, "mixed", 8, 16, 1), (cabi.INT8, "mixed", 8, 16, 1100), (cabi.F16, 1.0, 18, 2048, 1), (cabi.F16, 1.0, 18, 128, 1100),
+    (cabi.FP8_E4M3, 1.0, 18, 2048, 1), (cabi.BF16, 1.0, 18, 2048, 1)])
+def test_small_weights_beside_a_dominating_token_count(dev, dtype, vmag, lead, keep, T):
+    """A token that leads by many nats, and thousands whose weights -- int8: weight times V scale -- lie where fp16 ends:
+    together they hold a share of the output, and must not vanish in the product while the sum counts them."""
+    rng = np.random.default_rng(keep + T)
+    p = SinkPages(rng, dtype, lead, vmag)
+    sel = rng.integers(1, p.NB, keep).astype(np.int32)
+    sel[keep // 3] = 0
+    sels, q = np.tile(sel, (T, 1, 1)), np.tile(p.q, (T, 1, 1))
+    need = cabi.lib().drk_paged_sparse_workspace_bytes(C.byref(p.g), T, keep)
+    pieces = need // (T * p.QH * (p.D + 2) * 4) or 1
+    groups = keep * (p.bs // 16)
+    chain = 16 * math.ceil(groups / pieces / (8 if T == 1 else 1)) + 8 + pieces
+    want, tol = p.want(sel, chain)
+    do, dq, dp, dt, ds = U.dev_zeros(q.nbytes), U.dev_bytes(q), U.dev_bytes(p.raw), U.dev_i32(np.arange(p.NB)), U.dev_i32(sels)
+    ws = U.dev_zeros(need + 16)
+    cabi.call("drk_paged_sparse_attention", p.g, U.p(dq), U.p(dp), U.p(dt), 0, None, p.NB * p.bs - 1, T, U.p(ds), keep, U.p(do), 0,
+              1 / math.sqrt(p.D), p.io, None, 0, U.p(ws), need, U.stream_ptr())
+    U.sync()
+    got = U.from_bits(U.host(do, np.uint16, q.shape), p.io)
+    for t in {0, T // 2, T - 1}:
+        ok, r = R.attend_ok(got[t], want, tol, p.io)
+        assert ok, (t, r)

@@ -208,6 +208,7 @@ SIGNATURES = {
     "drk_block_select_workspace_bytes": (_sz, [_LP, _i32, _i32]),
     "drk_block_select": (_i32, [_LP, _vp, _i32, _vp, _i32, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
     "drk_paged_sparse_workspace_bytes": (_sz, [_LP, _i32, _i32]),
+    "drk_paged_sparse_check": (_i32, [_LP, _i32, _i32, _i32]),
     "drk_paged_sparse_attention": (_i32, [_LP, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _i32, _vp, _i32, _f32, _i32, _vp, _sz, _vp,
                                           _sz, _vp]),
 }

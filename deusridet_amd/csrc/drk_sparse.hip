@@ -505,6 +505,13 @@ static int sparse_check(const drk_kv_layout *g, Lay *a, int T, int n_keep, int *
     return DRK_OK;
 }
 
+static int sparse_check_io(const Lay &a, int io_dtype, const char *who)
+{
+    if (io_dtype != DRK_F16 && io_dtype != DRK_BF16) return fail(DRK_ERR_INVALID, "%s: io_dtype must be F16 or BF16", who);
+    if (a.E == 2 && io_dtype != a.dtype) return fail(DRK_ERR_INVALID, "%s: io_dtype %d differs from the pool's %d", who, io_dtype, a.dtype);
+    return DRK_OK;
+}
+
 static size_t sparse_need(const Lay &a, int T, int pieces)
 {
     return pieces > 1 ? (size_t)T * a.QH * pieces * (a.D + 2) * 4 : 0;
@@ -524,6 +531,14 @@ size_t drk_paged_sparse_workspace_bytes(const drk_kv_layout *g, int T, int n_kee
     return sparse_need(a, T, pieces);
 }
 
+int drk_paged_sparse_check(const drk_kv_layout *g, int T, int n_keep, int io_dtype)
+{
+    Lay a;
+    int pieces, gpp;
+    const int rc = sparse_check(g, &a, T, n_keep, &pieces, &gpp, "paged_sparse_check");
+    return rc ? rc : sparse_check_io(a, io_dtype, "paged_sparse_check");
+}
+
 int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void *pool, const int32_t *d_tables, int table_stride,
                                const int32_t *d_seq_lens, int pos_start, int T, const int32_t *d_selected, int n_keep, void *out,
                                int layer, float scale, int io_dtype, const void *gate, size_t gate_stride, void *workspace,
@@ -533,9 +548,8 @@ int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void
     SparseArgs A;
     int rc = sparse_check(g, &a, T, n_keep, &A.pieces, &A.groups_per_piece, "paged_sparse_attention");
     if (rc) return rc;
-    if (io_dtype != DRK_F16 && io_dtype != DRK_BF16) return fail(DRK_ERR_INVALID, "paged_sparse_attention: io_dtype must be F16 or BF16");
-    if (a.E == 2 && io_dtype != a.dtype)
-        return fail(DRK_ERR_INVALID, "paged_sparse_attention: io_dtype %d differs from the pool's %d", io_dtype, a.dtype);
+    rc = sparse_check_io(a, io_dtype, "paged_sparse_attention");
+    if (rc) return rc;
     if (layer < 0 || layer >= a.L) return fail(DRK_ERR_INVALID, "paged_sparse_attention: layer %d outside [0,%d)", layer, a.L);
     if (table_stride < 0 || pos_start < 0 || pos_start > 0x7fffffff - T || !(scale > 0.0f))
         return fail(DRK_ERR_INVALID, "paged_sparse_attention: bad argument");

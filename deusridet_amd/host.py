@@ -86,6 +86,8 @@ SIGNATURES = {
                                                          _i32, C.POINTER(_vp), _vp]),
     "drkh_paged_attention_release_workspace": (None, []),
     "drkh_apply_rope_scaled": (None, [C.POINTER(cabi.Rope)] + [_vp] * 3 + [_i32] * 4 + [_vp, _i32, _i32, _vp]),
+    "drkh_paged_sparse_attention_supported": (_i32, [_i32]),
+    "drkh_paged_sparse_workspace_bytes": (_sz, [_i32] * 5),
     "drkh_paged_prefill_sparse": (_i32, [_vp] * 4 + [_i32] * 5 + [_vp, _vp, _i32, _vp] + [_i32] * 3 + [_f32, _vp]),
     "drkh_kvs_create": (_vp, []),
     "drkh_kvs_destroy": (None, [_vp]),

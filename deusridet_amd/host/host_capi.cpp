@@ -245,6 +245,11 @@ void drkh_apply_rope_scaled(const drk_rope *rope, const double *d_freqs, void *q
 {
     apply_rope_scaled(*rope, d_freqs, H(q), H(k), T, num_heads, num_kv_heads, head_dim, d_pos, pos_start, inverse != 0, ST(stream));
 }
+int drkh_paged_sparse_attention_supported(int block_size) { return paged_sparse_attention_supported(block_size) ? 1 : 0; }
+size_t drkh_paged_sparse_workspace_bytes(int max_rows, int max_seq_len, int n_keep, int max_phys_blocks, int block_size)
+{
+    return paged_sparse_workspace_bytes(max_rows, max_seq_len, n_keep, max_phys_blocks, block_size);
+}
 int drkh_paged_prefill_sparse(const void *Q, const void *pool, void *d_bounds, const int32_t *d_block_table, int pos_start, int M,
                               int n_keep, int n_sink, int n_recent, int32_t *d_selected, const void *gate, int gate_stride,
                               void *out, int fa_layer_idx, int max_phys_blocks, int block_size, float scale, void *stream)

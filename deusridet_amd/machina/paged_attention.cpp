@@ -217,8 +217,8 @@ void paged_gqa_decode_attention_shared(AttentionWorkspace& ws, const __half* Q, 
 
 bool paged_sparse_attention_supported(int block_size)
 {
-    return (ModelConfig::HEAD_DIM == 128 || ModelConfig::HEAD_DIM == 256) && block_size > 0 && block_size % 16 == 0 &&
-           ModelConfig::NUM_KV_HEADS > 0 && ModelConfig::NUM_ATTN_HEADS / ModelConfig::NUM_KV_HEADS <= 16;
+    drk_kv_layout g = ModelConfig::layout(1, block_size);
+    return drk_paged_sparse_check(&g, 1, 1, ModelConfig::IO_DTYPE) == DRK_OK;
 }
 
 size_t paged_kv_bounds_bytes(int max_phys_blocks, int block_size)
@@ -233,6 +233,7 @@ size_t paged_sparse_workspace_bytes(int max_rows, int max_seq_len, int n_keep, i
     // the largest of every number of rows up to the most that are ever cut.
     drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
     size_t need = drk_block_select_workspace_bytes(&g, max_rows, max_seq_len);
+    if (need == 0 || drk_paged_sparse_check(&g, max_rows, n_keep, ModelConfig::IO_DTYPE) != DRK_OK) return 0;
     for (int rows = 1; rows <= max_rows && rows <= 512; rows++) {
         const size_t n = drk_paged_sparse_workspace_bytes(&g, rows, n_keep);
         need = n > need ? n : need;

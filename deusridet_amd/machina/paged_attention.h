@@ -236,10 +236,12 @@ void paged_gqa_decode_attention_branches_scored(AttentionWorkspace& ws, const vo
 // A decode step or a chunk behind a very long context reads the blocks whose keys can matter instead of all: the
 // bounds of every block's keys are kept beside the pool (update them after the write), a query scores the blocks
 // against their bounds and keeps the best, attention reads those.  drk_kv.h has the definitions.  HEAD_DIM 128 or 256,
-// block_size % 16 == 0, at most 16 query heads per kv head: check paged_sparse_attention_supported().
+// block_size % 16 == 0, at most 16 query heads per kv head, 16-bit pages of IO_DTYPE: check
+// paged_sparse_attention_supported().
 bool paged_sparse_attention_supported(int block_size);
 size_t paged_kv_bounds_bytes(int max_phys_blocks, int block_size);
-// Enough for the selection and the attention of up to max_rows rows, which may share it on one stream.
+// Enough for the selection and the attention of up to max_rows rows, which may share it on one stream; 0 where one of them
+// is refused (a list of more than 524 288 tokens, say).
 size_t paged_sparse_workspace_bytes(int max_rows, int max_seq_len, int n_keep, int max_phys_blocks, int block_size);
 // Recompute the bounds of the blocks that tokens pos_start .. pos_start + M - 1 of one table lie in, layers
 // fa_layer_idx .. + num_layers - 1; of the block of d_pos[b] of every branch b.

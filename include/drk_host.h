@@ -161,6 +161,8 @@ struct drk_rope;                 /* drk_kv.h */
  * and paged_prefill_attention_sparse (paged_attention.h) on a workspace of its own, waited for; 0 when that cannot be had */
 void drkh_apply_rope_scaled(const struct drk_rope *rope, const double *d_freqs, void *q, void *k, int T, int num_heads, int num_kv_heads,
                             int head_dim, const int32_t *d_pos, int pos_start, int inverse, void *stream);
+int  drkh_paged_sparse_attention_supported(int block_size);
+size_t drkh_paged_sparse_workspace_bytes(int max_rows, int max_seq_len, int n_keep, int max_phys_blocks, int block_size);
 int  drkh_paged_prefill_sparse(const void *Q, const void *pool, void *d_bounds, const int32_t *d_block_table, int pos_start, int M,
                                int n_keep, int n_sink, int n_recent, int32_t *d_selected, const void *gate, int gate_stride,
                                void *out, int fa_layer_idx, int max_phys_blocks, int block_size, float scale, void *stream);

@@ -564,9 +564,12 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
  * attention * sigmoid(gate) (rows gate_stride elements apart, 16-byte aligned), rounded once; a row without a token,
  * or whose every score is -inf, is left as it was.  head_dim 128 or 256, block_size % 16 == 0, at most 16 query heads per kv head, every storage
  * type (as the page's own type when it is 16 bits, io_dtype must equal it); DRK_ERR_UNSUPPORTED otherwise.
- * One layer of the pool holds at most 64 GiB.  Workspace for the pieces of rows that are cut:
+ * One layer of the pool holds at most 64 GiB, a list at most 524 288 tokens (n_keep * block_size).  Workspace for the pieces of rows that are cut:
  * drk_paged_sparse_workspace_bytes, 16-byte aligned, not cleared. */
 size_t drk_paged_sparse_workspace_bytes(const drk_kv_layout *g, int T, int n_keep);
+/* Whether the call takes T rows of n_keep blocks of this geometry and these types: DRK_OK, or what it would return
+ * (drk_paged_sparse_workspace_bytes is 0 both where nothing is needed and where the call is refused). */
+int drk_paged_sparse_check(const drk_kv_layout *g, int T, int n_keep, int io_dtype);
 int drk_paged_sparse_attention(const drk_kv_layout *g, const void *q, const void *pool, const int32_t *d_tables,
                                int table_stride, const int32_t *d_seq_lens, int pos_start, int T,
                                const int32_t *d_selected, int n_keep, void *out, int layer, float scale, int io_dtype,

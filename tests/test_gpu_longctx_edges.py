@@ -8,6 +8,8 @@ import pytest
 from deusridet_amd import cabi, host
 from tests import longctx_ref as R
 from tests import test_gpu_longctx as G
+from tests import test_gpu_stream as S
+from tests import test_gpu_stream_sparse as SP
 from tests import util as U
 
 pytestmark = pytest.mark.gpu
@@ -129,3 +131,28 @@ def test_small_weights_beside_a_dominating_token_count(dev, dtype, vmag, lead, k
     for t in {0, T // 2, T - 1}:
         ok, r = R.attend_ok(got[t], want, tol, p.io)
         assert ok, (t, r)
+
+
+# ---- through the host functions and the stream driver --------------------------------------------
+def test_the_driver_refuses_a_budget_that_the_attention_refuses(dev):
+    """More than 524 288 tokens a row: refused, and the policy in force stays as it is."""
+    s = S.Session(2)
+    st = U.stream_ptr()
+    most = 524288 // S.BS
+    assert not s.ks.set_sparse_decode(0, most + 1, 1, 2, st) and not s.ks.set_sparse_decode(0, 2 ** 30, 1, 2, st)
+    rng = np.random.default_rng(3)
+    s.set_weights(U.normal_bits(rng, (S.D,), S.DT), U.normal_bits(rng, (S.D,), S.DT))
+    assert s.ks.set_sparse_decode(0, 3, 1, 1, st)
+    SP.prefill(s, rng, (64, 50))
+    assert s.ks.open_branches(2) == 2
+    ids = [s.ks.branch_id(i) for i in range(2)]
+    for step in range(2):
+        assert not s.ks.set_sparse_decode(0, most + 1, 0, 0, st)
+        assert s.ks.begin_decode_step(st)
+        pos = [s.ks.branch_pos(i) for i in range(2)]
+        for layer, x in enumerate(SP.step_inputs(rng, 2)):
+            s.load(*x)
+            s.ks.decode_layer(layer, s.io(), st)
+            SP.check_step(s, layer, ids, pos, x[0], s.out(2), 3, 1, 1)
+        s.ks.end_decode_step(st)
+    assert s.ks.set_sparse_decode(0, most, 1, 2, st)

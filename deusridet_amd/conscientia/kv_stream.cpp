@@ -153,9 +153,9 @@ void KvStream::prefill_layer(int fa_layer_idx, const KvLayerIO& io, int M, hipSt
     paged_qk_norm_rope_write_batch(io.qg, io.k, io.v, io.q_norm, io.k_norm, io.q_scratch, pool.pool_ptr(),
                                    cm_->d_block_table(0), fa_layer_idx, current_pos_, M, pool.max_blocks(),
                                    pool.block_size(), d_rope_table_, table_positions_, stream);
-    if (d_bounds_)
-        paged_kv_bounds_update_batch(d_bounds_, pool.pool_ptr(), cm_->d_block_table(0), fa_layer_idx, 1, current_pos_, M,
-                                     pool.max_blocks(), pool.block_size(), stream);
+    if (d_bounds_ && !paged_kv_bounds_update_batch(d_bounds_, pool.pool_ptr(), cm_->d_block_table(0), fa_layer_idx, 1, current_pos_, M,
+                                                   pool.max_blocks(), pool.block_size(), stream))
+        bounds_current_ = false;
     if (!scored) {
         paged_prefill_attention_gated(ws_prefill_, io.q_scratch, pool.pool_ptr(), cm_->d_block_table(0), io.qg + hd, 2 * hd, io.attn_out,
                                       fa_layer_idx, current_pos_, M, pool.max_blocks(), pool.block_size(), scale, stream);
@@ -280,6 +280,20 @@ bool KvStream::set_sparse_decode(int min_tokens, int n_keep, int n_sink, int n_r
         LOG_ERROR("Conscientia", "KvStream: buffers of the block selection: %s", drk_last_error());
         return false;                                         // fresh frees itself
     }
+    // what is there already: the stream's own context and every open branch's.  Whatever stream wrote it has to be
+    // done, and the streams of the next steps find the bounds there.
+    bool filled = drk_device_synchronize() == DRK_OK;
+    cm_->sync_block_table(stream);
+    filled = filled && paged_kv_bounds_update_batch(p, pool.pool_ptr(), cm_->d_block_table(0), 0, ModelConfig::NUM_FA_LAYERS, 0,
+                                                    current_pos_, nb, bs, stream);
+    for (size_t i = 0; filled && i < branches_.size(); i++)
+        filled = paged_kv_bounds_update_batch(p, pool.pool_ptr(), cm_->d_block_table(branches_[i]), 0, ModelConfig::NUM_FA_LAYERS, 0, pos_[i],
+                                              nb, bs, stream);
+    if (drk_stream_synchronize(stream) != DRK_OK || !filled) {
+        LOG_ERROR("Conscientia", "KvStream: reading the context's bounds: %s", drk_last_error());
+        drk_dev_free(p);
+        return false;
+    }
     drop_graph();
     drop_sparse();
     ws_sparse_.adopt(fresh);
@@ -289,16 +303,7 @@ bool KvStream::set_sparse_decode(int min_tokens, int n_keep, int n_sink, int n_r
     sparse_keep_ = n_keep;
     sparse_sink_ = n_sink;
     sparse_recent_ = n_recent;
-    // what is there already: the stream's own context and every open branch's.  Whatever stream wrote it has to be
-    // done, and the streams of the next steps find the bounds there.
-    drk_device_synchronize();
-    cm_->sync_block_table(stream);
-    paged_kv_bounds_update_batch(d_bounds_, pool.pool_ptr(), cm_->d_block_table(0), 0, ModelConfig::NUM_FA_LAYERS, 0, current_pos_, nb, bs,
-                                 stream);
-    for (size_t i = 0; i < branches_.size(); i++)
-        paged_kv_bounds_update_batch(d_bounds_, pool.pool_ptr(), cm_->d_block_table(branches_[i]), 0, ModelConfig::NUM_FA_LAYERS, 0,
-                                     pos_[i], nb, bs, stream);
-    if (drk_stream_synchronize(stream) != DRK_OK) LOG_ERROR("Conscientia", "KvStream: reading the context's bounds: %s", drk_last_error());
+    bounds_current_ = true;
     return true;
 }
 
@@ -404,18 +409,20 @@ void KvStream::decode_layer(int fa_layer_idx, const KvLayerIO& io, hipStream_t s
                                       d_pos_, B, fa_layer_idx, pool.max_blocks(), pool.block_size(), d_rope_table_,
                                       table_positions_, stream);
     const __half* gate = io.qg + hd;
-    if (d_bounds_)
-        paged_kv_bounds_update_branches(d_bounds_, pool.pool_ptr(), tables, stride, d_pos_, B, fa_layer_idx, 1, pool.max_blocks(),
-                                        pool.block_size(), stream);
+    if (d_bounds_ && !paged_kv_bounds_update_branches(d_bounds_, pool.pool_ptr(), tables, stride, d_pos_, B, fa_layer_idx, 1,
+                                                      pool.max_blocks(), pool.block_size(), stream))
+        bounds_current_ = false;
     int min_len = pos_[0] + 1;
     for (int p : pos_) min_len = p + 1 < min_len ? p + 1 : min_len;
-    if (d_bounds_ && min_len >= sparse_min_tokens_) {
+    // a refused call leaves the layer to the whole-context paths below
+    if (d_bounds_ && bounds_current_ && min_len >= sparse_min_tokens_ &&
         paged_block_select_branches(ws_sparse_, d_bounds_, io.q_scratch, tables, stride, d_len_, B, max_len, sparse_keep_, sparse_sink_,
-                                    sparse_recent_, d_selected_, fa_layer_idx, pool.max_blocks(), pool.block_size(), stream);
+                                    sparse_recent_, d_selected_, fa_layer_idx, pool.max_blocks(), pool.block_size(), stream) &&
         paged_gqa_decode_attention_sparse(ws_sparse_, io.q_scratch, pool.pool_ptr(), tables, stride, d_len_, B, d_selected_,
                                           sparse_keep_, gate, 2 * hd, io.attn_out, fa_layer_idx, pool.max_blocks(),
-                                          pool.block_size(), scale, stream);
-    } else if (scorer_ && scorer_->d_new_scores()) {
+                                          pool.block_size(), scale, stream))
+        return;
+    if (scorer_ && scorer_->d_new_scores()) {
         if (first_layer_of_step_ < 0) first_layer_of_step_ = fa_layer_idx;
         float* mass = scorer_->d_new_scores() + (size_t)branches_[0] * stride;
         // the step's unit descriptors where the kernel takes a plan, the gate on the merge

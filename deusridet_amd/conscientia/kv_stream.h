@@ -95,9 +95,10 @@ public:
     // keys -- instead of the whole context.  The bounds are kept from here on (perception and decode update them
     // behind their writes; what the open branches and the stream hold already is read once, and waited for).  n_keep 0
     // turns it off and frees the buffers.  False, and nothing changes, where the kernels do not take the geometry,
-    // with a scorer attached (it wants the attention mass of every block), with an overflow tier (a block that comes
-    // back may have lost its bounds), or when the device allocation fails.  Takes precedence over the shared-prefix
-    // paths.  Call it between steps; a captured step is dropped, and one captured afterwards keeps the path --
+    // or the budget (524 288 tokens a row at most), with a scorer attached (it wants the attention mass of every block),
+    // with an overflow tier (a block that comes back may have lost its bounds), or when the allocation or the reading
+    // fails.  Takes precedence over the shared-prefix paths; a layer whose calls are refused reads the whole context.
+    // Call it between steps; a captured step is dropped, and one captured afterwards keeps the path --
     // selected or whole -- its branches' lengths called for when it was captured.
     bool set_sparse_decode(int min_tokens, int n_keep, int n_sink, int n_recent, hipStream_t stream = nullptr);
 
@@ -156,6 +157,7 @@ private:
 
     // decode over selected blocks: one allocation holds the bounds and the selection
     void* d_bounds_ = nullptr;
+    bool bounds_current_ = false;          // no update of them was refused
     int* d_selected_ = nullptr;            // [max_branches][kv heads][sparse_keep_]
     AttentionWorkspace ws_sparse_;
     int sparse_min_tokens_ = 0, sparse_keep_ = 0, sparse_sink_ = 0, sparse_recent_ = 0;

@@ -257,12 +257,13 @@ int drkh_paged_prefill_sparse(const void *Q, const void *pool, void *d_bounds, c
     AttentionWorkspace ws;
     const size_t need = paged_sparse_workspace_bytes(M, pos_start + M, n_keep, max_phys_blocks, block_size);
     if (need == 0 || !ws.reserve(need)) return 0;
-    paged_kv_bounds_update_batch(d_bounds, CH(pool), d_block_table, fa_layer_idx, 1, 0, pos_start + M, max_phys_blocks, block_size, ST(stream));
-    paged_block_select_prefill(ws, d_bounds, CH(Q), d_block_table, pos_start, M, n_keep, n_sink, n_recent, d_selected, fa_layer_idx,
-                               max_phys_blocks, block_size, ST(stream));
-    paged_prefill_attention_sparse(ws, CH(Q), CH(pool), d_block_table, d_selected, n_keep, CH(gate), gate_stride, H(out), fa_layer_idx,
-                                   pos_start, M, max_phys_blocks, block_size, scale, ST(stream));
-    return drk_stream_synchronize(stream) == DRK_OK ? 1 : 0;
+    const bool ok =
+        paged_kv_bounds_update_batch(d_bounds, CH(pool), d_block_table, fa_layer_idx, 1, 0, pos_start + M, max_phys_blocks, block_size, ST(stream)) &&
+        paged_block_select_prefill(ws, d_bounds, CH(Q), d_block_table, pos_start, M, n_keep, n_sink, n_recent, d_selected, fa_layer_idx,
+                                   max_phys_blocks, block_size, ST(stream)) &&
+        paged_prefill_attention_sparse(ws, CH(Q), CH(pool), d_block_table, d_selected, n_keep, CH(gate), gate_stride, H(out), fa_layer_idx,
+                                       pos_start, M, max_phys_blocks, block_size, scale, ST(stream));
+    return drk_stream_synchronize(stream) == DRK_OK && ok ? 1 : 0;                // waited for either way: the workspace ends here
 }
 void drkh_head_norm(const void *x, const void *weight, void *out, int num_heads, int head_dim, float eps,
                     void *stream)

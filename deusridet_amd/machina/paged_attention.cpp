@@ -242,76 +242,88 @@ size_t paged_sparse_workspace_bytes(int max_rows, int max_seq_len, int n_keep, i
     return n > need ? n : need;
 }
 
-void paged_kv_bounds_update_batch(void* d_bounds, const __half* kv_pool, const int* d_block_table, int fa_layer_idx,
+bool paged_kv_bounds_update_batch(void* d_bounds, const __half* kv_pool, const int* d_block_table, int fa_layer_idx,
                                   int num_layers, int pos_start, int M, int max_phys_blocks, int block_size, hipStream_t stream)
 {
-    if (M <= 0) return;
+    if (M <= 0) return true;
     drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
-    if (drk_kv_bounds_update(&g, kv_pool, d_block_table, 0, nullptr, pos_start, M, fa_layer_idx, num_layers, d_bounds, stream) != DRK_OK)
-        LOG_ERROR("Machina", "paged_kv_bounds_update_batch: %s", drk_last_error());
+    if (drk_kv_bounds_update(&g, kv_pool, d_block_table, 0, nullptr, pos_start, M, fa_layer_idx, num_layers, d_bounds, stream) == DRK_OK) return true;
+    LOG_ERROR("Machina", "paged_kv_bounds_update_batch: %s", drk_last_error());
+    return false;
 }
 
-void paged_kv_bounds_update_branches(void* d_bounds, const __half* kv_pool, const int* d_tables, int table_stride,
+bool paged_kv_bounds_update_branches(void* d_bounds, const __half* kv_pool, const int* d_tables, int table_stride,
                                      const int* d_pos, int B, int fa_layer_idx, int num_layers, int max_phys_blocks,
                                      int block_size, hipStream_t stream)
 {
-    if (B <= 0) return;
+    if (B <= 0) return true;
     drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
     if (!d_pos)
         LOG_ERROR("Machina", "paged_kv_bounds_update_branches: d_pos is null");
-    else if (drk_kv_bounds_update(&g, kv_pool, d_tables, table_stride, d_pos, 0, B, fa_layer_idx, num_layers, d_bounds, stream) != DRK_OK)
+    else if (drk_kv_bounds_update(&g, kv_pool, d_tables, table_stride, d_pos, 0, B, fa_layer_idx, num_layers, d_bounds, stream) == DRK_OK)
+        return true;
+    else
         LOG_ERROR("Machina", "paged_kv_bounds_update_branches: %s", drk_last_error());
+    return false;
 }
 
-void paged_block_select_branches(AttentionWorkspace& ws, const void* d_bounds, const __half* Q, const int* d_tables,
+bool paged_block_select_branches(AttentionWorkspace& ws, const void* d_bounds, const __half* Q, const int* d_tables,
                                  int table_stride, const int* d_seq_lens, int B, int max_seq_len, int n_keep, int n_sink,
                                  int n_recent, int* d_selected, int fa_layer_idx, int max_phys_blocks, int block_size,
                                  hipStream_t stream)
 {
-    if (B <= 0) return;
+    if (B <= 0) return true;
     drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
     if (!d_seq_lens)
         LOG_ERROR("Machina", "paged_block_select_branches: d_seq_lens is null");
     else if (drk_block_select(&g, d_bounds, fa_layer_idx, Q, ModelConfig::IO_DTYPE, d_tables, table_stride, d_seq_lens, 0, B,
-                              max_seq_len, n_keep, n_sink, n_recent, d_selected, ws.ptr(), ws.bytes(), stream) != DRK_OK)
+                              max_seq_len, n_keep, n_sink, n_recent, d_selected, ws.ptr(), ws.bytes(), stream) == DRK_OK)
+        return true;
+    else
         LOG_ERROR("Machina", "paged_block_select_branches: %s", drk_last_error());
+    return false;
 }
 
-void paged_block_select_prefill(AttentionWorkspace& ws, const void* d_bounds, const __half* Q, const int* d_block_table,
+bool paged_block_select_prefill(AttentionWorkspace& ws, const void* d_bounds, const __half* Q, const int* d_block_table,
                                 int pos_start, int M, int n_keep, int n_sink, int n_recent, int* d_selected,
                                 int fa_layer_idx, int max_phys_blocks, int block_size, hipStream_t stream)
 {
-    if (M <= 0) return;
+    if (M <= 0) return true;
     drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
     if (drk_block_select(&g, d_bounds, fa_layer_idx, Q, ModelConfig::IO_DTYPE, d_block_table, 0, nullptr, pos_start, M, pos_start + M,
-                         n_keep, n_sink, n_recent, d_selected, ws.ptr(), ws.bytes(), stream) != DRK_OK)
-        LOG_ERROR("Machina", "paged_block_select_prefill: %s", drk_last_error());
+                         n_keep, n_sink, n_recent, d_selected, ws.ptr(), ws.bytes(), stream) == DRK_OK) return true;
+    LOG_ERROR("Machina", "paged_block_select_prefill: %s", drk_last_error());
+    return false;
 }
 
-void paged_gqa_decode_attention_sparse(AttentionWorkspace& ws, const __half* Q, const __half* kv_pool, const int* d_tables,
+bool paged_gqa_decode_attention_sparse(AttentionWorkspace& ws, const __half* Q, const __half* kv_pool, const int* d_tables,
                                        int table_stride, const int* d_seq_lens, int B, const int* d_selected, int n_keep,
                                        const __half* gate, int gate_stride, __half* out, int fa_layer_idx, int max_phys_blocks,
                                        int block_size, float scale, hipStream_t stream)
 {
-    if (B <= 0) return;
+    if (B <= 0) return true;
     drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
     if (!d_seq_lens)
         LOG_ERROR("Machina", "paged_gqa_decode_attention_sparse: d_seq_lens is null");
     else if (drk_paged_sparse_attention(&g, Q, kv_pool, d_tables, table_stride, d_seq_lens, 0, B, d_selected, n_keep, out, fa_layer_idx,
-                                        scale, ModelConfig::IO_DTYPE, gate, (size_t)gate_stride, ws.ptr(), ws.bytes(), stream) != DRK_OK)
+                                        scale, ModelConfig::IO_DTYPE, gate, (size_t)gate_stride, ws.ptr(), ws.bytes(), stream) == DRK_OK)
+        return true;
+    else
         LOG_ERROR("Machina", "paged_gqa_decode_attention_sparse: %s", drk_last_error());
+    return false;
 }
 
-void paged_prefill_attention_sparse(AttentionWorkspace& ws, const __half* Q, const __half* kv_pool, const int* d_block_table,
+bool paged_prefill_attention_sparse(AttentionWorkspace& ws, const __half* Q, const __half* kv_pool, const int* d_block_table,
                                     const int* d_selected, int n_keep, const __half* gate, int gate_stride, __half* out,
                                     int fa_layer_idx, int pos_start, int M, int max_phys_blocks, int block_size, float scale,
                                     hipStream_t stream)
 {
-    if (M <= 0) return;
+    if (M <= 0) return true;
     drk_kv_layout g = ModelConfig::layout(max_phys_blocks, block_size);
     if (drk_paged_sparse_attention(&g, Q, kv_pool, d_block_table, 0, nullptr, pos_start, M, d_selected, n_keep, out, fa_layer_idx, scale,
-                                   ModelConfig::IO_DTYPE, gate, (size_t)gate_stride, ws.ptr(), ws.bytes(), stream) != DRK_OK)
-        LOG_ERROR("Machina", "paged_prefill_attention_sparse: %s", drk_last_error());
+                                   ModelConfig::IO_DTYPE, gate, (size_t)gate_stride, ws.ptr(), ws.bytes(), stream) == DRK_OK) return true;
+    LOG_ERROR("Machina", "paged_prefill_attention_sparse: %s", drk_last_error());
+    return false;
 }
 
 size_t paged_decode_plan_bytes(int B, int max_seq_len, int max_phys_blocks, int block_size, int n_groups)

@@ -243,28 +243,29 @@ size_t paged_kv_bounds_bytes(int max_phys_blocks, int block_size);
 // Enough for the selection and the attention of up to max_rows rows, which may share it on one stream; 0 where one of them
 // is refused (a list of more than 524 288 tokens, say).
 size_t paged_sparse_workspace_bytes(int max_rows, int max_seq_len, int n_keep, int max_phys_blocks, int block_size);
+// The six calls below say whether they were taken: where one was refused (logged) nothing was launched.
 // Recompute the bounds of the blocks that tokens pos_start .. pos_start + M - 1 of one table lie in, layers
 // fa_layer_idx .. + num_layers - 1; of the block of d_pos[b] of every branch b.
-void paged_kv_bounds_update_batch(void* d_bounds, const __half* kv_pool, const int* d_block_table, int fa_layer_idx,
+bool paged_kv_bounds_update_batch(void* d_bounds, const __half* kv_pool, const int* d_block_table, int fa_layer_idx,
                                   int num_layers, int pos_start, int M, int max_phys_blocks, int block_size,
                                   hipStream_t stream = 0);
-void paged_kv_bounds_update_branches(void* d_bounds, const __half* kv_pool, const int* d_tables, int table_stride,
+bool paged_kv_bounds_update_branches(void* d_bounds, const __half* kv_pool, const int* d_tables, int table_stride,
                                      const int* d_pos, int B, int fa_layer_idx, int num_layers, int max_phys_blocks,
                                      int block_size, hipStream_t stream = 0);
 // d_selected [B or M][NUM_KV_HEADS][n_keep]: the first n_sink and the last n_recent blocks of a row and the best others.
-void paged_block_select_branches(AttentionWorkspace& ws, const void* d_bounds, const __half* Q, const int* d_tables,
+bool paged_block_select_branches(AttentionWorkspace& ws, const void* d_bounds, const __half* Q, const int* d_tables,
                                  int table_stride, const int* d_seq_lens, int B, int max_seq_len, int n_keep, int n_sink,
                                  int n_recent, int* d_selected, int fa_layer_idx, int max_phys_blocks, int block_size,
                                  hipStream_t stream = 0);
-void paged_block_select_prefill(AttentionWorkspace& ws, const void* d_bounds, const __half* Q, const int* d_block_table,
+bool paged_block_select_prefill(AttentionWorkspace& ws, const void* d_bounds, const __half* Q, const int* d_block_table,
                                 int pos_start, int M, int n_keep, int n_sink, int n_recent, int* d_selected,
                                 int fa_layer_idx, int max_phys_blocks, int block_size, hipStream_t stream = 0);
 // gate may be null; otherwise rows gate_stride elements apart, applied before the one rounding of the output.
-void paged_gqa_decode_attention_sparse(AttentionWorkspace& ws, const __half* Q, const __half* kv_pool, const int* d_tables,
+bool paged_gqa_decode_attention_sparse(AttentionWorkspace& ws, const __half* Q, const __half* kv_pool, const int* d_tables,
                                        int table_stride, const int* d_seq_lens, int B, const int* d_selected, int n_keep,
                                        const __half* gate, int gate_stride, __half* out, int fa_layer_idx,
                                        int max_phys_blocks, int block_size, float scale, hipStream_t stream = 0);
-void paged_prefill_attention_sparse(AttentionWorkspace& ws, const __half* Q, const __half* kv_pool, const int* d_block_table,
+bool paged_prefill_attention_sparse(AttentionWorkspace& ws, const __half* Q, const __half* kv_pool, const int* d_block_table,
                                     const int* d_selected, int n_keep, const __half* gate, int gate_stride, __half* out,
                                     int fa_layer_idx, int pos_start, int M, int max_phys_blocks, int block_size,
                                     float scale, hipStream_t stream = 0);

@@ -158,7 +158,8 @@ void drkh_paged_prefill_attention_gated(const void *Q, void *kv_pool, const int3
                                         int max_phys_blocks, int block_size, float scale, void *stream);
 struct drk_rope;                 /* drk_kv.h */
 /* apply_rope_scaled (layer.h); a chunk of M tokens over selected blocks: paged_kv_bounds_update_batch, paged_block_select_prefill
- * and paged_prefill_attention_sparse (paged_attention.h) on a workspace of its own, waited for; 0 when that cannot be had */
+ * and paged_prefill_attention_sparse (paged_attention.h) on a workspace of its own, waited for; 0 when that cannot be had or one of
+ * the three is refused (those behind it are not made) */
 void drkh_apply_rope_scaled(const struct drk_rope *rope, const double *d_freqs, void *q, void *k, int T, int num_heads, int num_kv_heads,
                             int head_dim, const int32_t *d_pos, int pos_start, int inverse, void *stream);
 int  drkh_paged_sparse_attention_supported(int block_size);

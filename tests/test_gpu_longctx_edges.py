@@ -156,3 +156,29 @@ def test_the_driver_refuses_a_budget_that_the_attention_refuses(dev):
             SP.check_step(s, layer, ids, pos, x[0], s.out(2), 3, 1, 1)
         s.ks.end_decode_step(st)
     assert s.ks.set_sparse_decode(0, most, 1, 2, st)
+
+
+@pytest.mark.parametrize("what", ["bounds", "selection", "attention"])
+def test_a_chunk_whose_call_is_refused_says_so(dev, what):
+    """drkh_paged_prefill_sparse is 0 where one of its three calls is refused, and those behind it are not made."""
+    D, QH, KVH, bs, start, M, keep = 128, 8, 2, 16, 60, 9, 3
+    assert host.set_attention_geometry(1, QH, KVH, D, cabi.BF16, cabi.BF16)
+    rng = np.random.default_rng(1)
+    p = R.Pool(rng, 1, KVH, QH, D, bs, 8, cabi.BF16)
+    q = U.normal_bits(rng, (M, QH, D), cabi.BF16)
+    dq, dp, dt, db = U.dev_bytes(q), U.dev_bytes(p.raw), U.dev_i32(np.arange(8)), U.dev_zeros(cabi.lib().drk_kv_bounds_bytes(C.byref(p.g)) + 16)
+    dsel, do = U.dev_i32(np.full((M, KVH, keep), 77)), U.dev_bytes(np.full(q.shape, 0x1234, np.uint16))
+
+    def call(refused):
+        bounds = db.data_ptr() + (8 if refused and what == "bounds" else 0)
+        sink = keep + 1 if refused and what == "selection" else 1
+        gate, stride = (U.p(dq), D // 2) if refused and what == "attention" else (None, 0)
+        return host.lib().drkh_paged_prefill_sparse(U.p(dq), U.p(dp), bounds, U.p(dt), start, M, keep, sink, 1, U.p(dsel), gate, stride, U.p(do),
+                                                    0, 8, bs, 1 / math.sqrt(D), U.stream_ptr())
+
+    assert call(True) == 0
+    assert (U.host(do, np.uint16) == 0x1234).all()
+    assert (U.host(dsel, np.int32) == 77).all() == (what != "attention") and U.host(db, np.uint8).any() == (what != "bounds")
+    assert call(False) == 1
+    sel = U.host(dsel, np.int32, (M, KVH, keep))
+    G.check_attend(p, U.host(do, np.uint16, q.shape), q, np.arange(8), start + 1 + np.arange(M), sel, cabi.BF16)

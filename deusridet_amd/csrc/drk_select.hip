@@ -39,6 +39,7 @@ constexpr size_t kSelFusedBytes = 200 << 10;   // codes of the context per kv he
 constexpr int kSelFusedRows = 256;             // (row, kv head) pairs that keep every CU busy by themselves
 constexpr int kSelFused = 1024;                // blocks, the most that kernel takes
 constexpr int kSelShort = 128;                 // blocks up to which chunks take it too, and fewer threads do
+constexpr int kSelWaveGroups = 4;              // 16-block groups of a wave of score_kernel: 64 table entries
 constexpr size_t kSelWaves = 4096;             // waves that a decode step's scores are spread over
 constexpr unsigned kSelTileWgs = 256;          // CUs that a chunk's workgroups are spread over
 constexpr unsigned kSelTileStart = 6;          // what such a workgroup spends on its queries, counted in groups
@@ -252,7 +253,8 @@ __device__ __forceinline__ void sel_wave_order()
 #endif
 }
 
-// One set of 16 heads per wave: a branch's row (R = 1), or R = 16 / P rows of one table.
+// One set of 16 heads per wave: a branch's row (R = 1), or R = 16 / P rows of one table.  A wave takes at most
+// kSelWaveGroups groups of 16 blocks: their table entries are its lanes' one load.
 template <int D>
 __global__ __launch_bounds__(256) void score_kernel(Lay a, SelArgs A)
 {
@@ -268,7 +270,7 @@ __global__ __launch_bounds__(256) void score_kernel(Lay a, SelArgs A)
     const int nbr = row < A.T ? sel_blocks_of_row(A, row) : 0;
     const int nbmax = max(max(__shfl(nbr, 0), __shfl(nbr, 16)), max(__shfl(nbr, 32), __shfl(nbr, 48)));
     if (first * 16 >= nbmax) return;
-    int ahead = first * 16 + lane < nbmax ? tab[first * 16 + lane] : -1;       // the table entries of four groups
+    const int ahead = first * 16 + lane < nbmax ? tab[first * 16 + lane] : -1;  // the table entries of all its groups
 
     const int qrow = min(A.R > 1 ? row0 + c / A.P : row0, A.T - 1);
     sel_i32x4 qa[KS];
@@ -279,9 +281,9 @@ __global__ __launch_bounds__(256) void score_kernel(Lay a, SelArgs A)
 
     sel_i32x4 bv[KS];
     int eb = 0;
-    auto fetch = [&](int i) {                                                   // group first + i; ahead holds its entries
-        sel_fetch<D>(bv, A.bounds, a, h, ahead, (i & 3) * 16, lane);
-        const int blk = __shfl(ahead, (i & 3) * 16 + c);
+    auto fetch = [&](int i) {                                                   // group first + i
+        sel_fetch<D>(bv, A.bounds, a, h, ahead, i * 16, lane);
+        const int blk = __shfl(ahead, i * 16 + c);
         eb = (unsigned)blk < (unsigned)a.NB ? (int)(int8_t)A.exps[(size_t)blk * a.KVH + h] : kNoBlock;
     };
     fetch(0);
@@ -291,13 +293,7 @@ __global__ __launch_bounds__(256) void score_kernel(Lay a, SelArgs A)
         sel_stage<D>(codes[w], bv, lane);
         sel_wave_order();
         const int e = eb;
-        if (i + 1 < n) {
-            if (((i + 1) & 3) == 0) {
-                const int at = (first + i + 1) * 16 + lane;
-                ahead = at < nbmax ? tab[at] : -1;
-            }
-            fetch(i + 1);
-        }
+        if (i + 1 < n) fetch(i + 1);
         sel_i32x4 acc = {0, 0, 0, 0};
 #if defined(__HIP_DEVICE_COMPILE__)
 #pragma unroll
@@ -864,8 +860,8 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
         } else {
             const size_t units = a.D <= 128 ? kSelWaves : kSelWaves / 2;          // as many waves as should have work of their own
             const size_t gpw = (all + units - 1) / units;
-            // a wave's first load covers the table entries of four groups: 16 branches x 64k, 4 groups 33.5 us, 8 groups 35.7
-            A.groups_per_wave = (int)(gpw > 4 ? 4 : gpw);
+            // (eight groups, with a second load of table entries: 16 branches x 64k 33.5 -> 35.7 us)
+            A.groups_per_wave = (int)(gpw > kSelWaveGroups ? kSelWaveGroups : gpw);
         }
         const size_t per = (size_t)A.groups_per_wave * (tile ? 1 : 4);
         const dim3 grid(a.KVH, (unsigned)((groups + per - 1) / per), (unsigned)tiles);

@@ -853,7 +853,6 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
     if (n > 0) {
         const int rows = tile ? 16 * A.R : A.R;
         const size_t tiles = ((size_t)T + rows - 1) / rows, groups = ((size_t)n + 15) / 16;
-        if (tiles > 65535 || groups > 65535) return fail(DRK_ERR_UNSUPPORTED, "block_select: %d rows are more than one launch takes", T);
         const size_t all = groups * a.KVH * tiles;                        // 16-block groups of every kv head and row tile
         if (tile) {
             A.groups_per_wave = sel_tile_groups(a, (unsigned)groups, (unsigned)(tiles * a.KVH));
@@ -864,7 +863,10 @@ int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, cons
             A.groups_per_wave = (int)(gpw > kSelWaveGroups ? kSelWaveGroups : gpw);
         }
         const size_t per = (size_t)A.groups_per_wave * (tile ? 1 : 4);
-        const dim3 grid(a.KVH, (unsigned)((groups + per - 1) / per), (unsigned)tiles);
+        const size_t parts = (groups + per - 1) / per;
+        if (tiles > 65535 || parts > 65535)
+            return fail(DRK_ERR_UNSUPPORTED, "block_select: %d rows of %d blocks are more than one launch takes", T, n);
+        const dim3 grid(a.KVH, (unsigned)parts, (unsigned)tiles);
         switch (a.D) {
         case 64: launch_score<64>(a, A, tile, grid, st); break;
         case 128: launch_score<128>(a, A, tile, grid, st); break;

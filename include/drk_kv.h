@@ -549,8 +549,10 @@ int drk_kv_bounds_extract(const drk_kv_layout *g, void *d_dst, const void *bound
  * -- (up to the rounding of q) an upper bound of every logit the block can give.  It is a whole number below 2^24
  * times a power of two: exact in 32 bits, the same for any order of summation.  NaN in q counts as 0.
  * max_seq_len bounds every row's length (a longer one is cut to it, as it is to the table_stride blocks of a table
- * row) and sizes the workspace, which need not be cleared: drk_block_select_workspace_bytes, 16-byte aligned.  1 <= n_keep, n_sink + n_recent <= n_keep; at most 16
- * query heads per kv head; head_dim as for the bounds; io_dtype DRK_F16 / DRK_BF16.  Rows of length <= 0 get -1. */
+ * row) and sizes the workspace, which need not be cleared: drk_block_select_workspace_bytes, 16-byte aligned.
+ * 1 <= n_keep, n_sink + n_recent <= n_keep; at most 16 query heads per kv head; head_dim as for the bounds; io_dtype
+ * DRK_F16 / DRK_BF16.  Rows of length <= 0 get -1.  DRK_ERR_UNSUPPORTED where one launch does not take the call: contexts up
+ * to 16 million blocks and 65 535 rows always fit. */
 size_t drk_block_select_workspace_bytes(const drk_kv_layout *g, int T, int max_seq_len);
 int drk_block_select(const drk_kv_layout *g, const void *bounds, int layer, const void *q, int io_dtype,
                      const int32_t *d_tables, int table_stride, const int32_t *d_seq_lens, int pos_start, int T,

@@ -182,3 +182,30 @@ def test_a_chunk_whose_call_is_refused_says_so(dev, what):
     assert call(False) == 1
     sel = U.host(dsel, np.int32, (M, KVH, keep))
     G.check_attend(p, U.host(do, np.uint16, q.shape), q, np.arange(8), start + 1 + np.arange(M), sel, cabi.BF16)
+
+
+# ---- selection ----------------------------------------------------------------------------------
+@pytest.mark.parametrize("T,mode", [(1, "branches"), (2, "branches"), (3, "one table"), (70, "one table")])
+def test_select_from_more_than_a_million_blocks(dev, T, mode):
+    """1.1 million blocks of one token (the pages repeat): every row's best ones, by the lower index among equals."""
+    rng = np.random.default_rng(T)
+    D, QH, KVH, bs, NB, n, keep, sink, recent, io = 64, 4, 1, 1, 5000, 1_100_003, 40, 2, 3, cabi.BF16
+    g = cabi.layout(1, KVH, QH, D, bs, NB, io)
+    codes, exps = R.bounds_buffers(1, NB, KVH, D, rng)
+    rows = T if mode == "branches" else 1
+    tables = rng.integers(0, NB, (rows, n)).astype(np.int32)
+    tables[:, 7] = -1
+    lens = n - rng.integers(0, 90000, T).astype(np.int32)
+    q = U.normal_bits(rng, (T, QH, D), io)
+    got = G.run_select(g, R.bounds_bytes(codes, exps), q, tables, n if mode == "branches" else 0, lens, 0, T, n, keep, sink, recent, io)
+    lo, hi = codes[0, :, 0].astype(np.int64).transpose(1, 0, 2)
+    for t in range(T) if T < 8 else (0, 33, T - 1):
+        score = np.full(NB, -np.inf)
+        for x in U.from_bits(q[t], io).astype(np.float64):
+            c, e = R.query_codes(x)
+            score = np.maximum(score, np.maximum(c * lo, c * hi).sum(1) * 2.0 ** (exps[0, :, 0].astype(np.float64) + e))
+        tab = tables[t if mode == "branches" else 0][:lens[t]]
+        s = np.where(tab >= 0, score[tab], -np.inf)
+        s[:sink], s[lens[t] - recent:] = np.inf, np.inf
+        want = np.sort(np.lexsort((np.arange(len(s)), -s))[:keep])
+        assert np.array_equal(got[t, 0], want), t

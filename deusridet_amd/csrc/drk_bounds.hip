@@ -296,6 +296,10 @@ int drk_kv_bounds_update(const drk_kv_layout *g, const void *pool, const int32_t
     A.bs_div = mk_div((unsigned)a.bs);
     A.first_block = d_pos ? 0 : pos_start / a.bs;
     A.n_blocks = d_pos ? n : (pos_start + n - 1) / a.bs - A.first_block + 1;
+    if (!d_pos && table_stride > 0 && A.n_blocks > table_stride - A.first_block) {      // what lies behind the table's row has no page
+        if (A.first_block >= table_stride) return DRK_OK;
+        A.n_blocks = table_stride - A.first_block;
+    }
     const size_t units = (size_t)A.n_blocks * a.KVH * layer_count;
     if (units * (a.row_bytes / 16) > ((size_t)0x7fffffff << 8) || units > 0x7fffffffu) return fail(DRK_ERR_INVALID, "kv_bounds_update: too many blocks");
     A.units = (unsigned)units;

@@ -528,7 +528,8 @@ size_t drk_kv_bounds_bytes(const drk_kv_layout *g);
  * d_pos != NULL: one token for each of n branches, at d_pos[i] of table row i * table_stride (0: one table for all, which
  * every position lies in) -- the block of d_pos[i] is covered up to d_pos[i] (a negative position, one behind the
  * table_stride blocks of its row, or a missing page is skipped).  NULL: tokens [pos_start, pos_start + n) of one table --
- * their blocks, up to pos_start + n - 1.  Tokens before pos_start in the first block count: the block is recomputed,
+ * their blocks, up to pos_start + n - 1; table_stride, where it is not 0, is the table's length in blocks, and tokens behind
+ * it are skipped.  Tokens before pos_start in the first block count: the block is recomputed,
  * not added to, so copies made on write, reused pages and rewritten positions need nothing special.  Two branches at
  * different positions of one physical block, which the append does not allow either, leave its bounds undefined. */
 int drk_kv_bounds_update(const drk_kv_layout *g, const void *pool, const int32_t *d_tables, int table_stride,

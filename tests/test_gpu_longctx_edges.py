@@ -41,6 +41,26 @@ def test_bounds_of_branches_over_one_table(dev, dtype, bs):
                 assert (codes[layer, blk] == 0x55).all() and (exps[layer, blk] == 0x55).all()
 
 
+@pytest.mark.parametrize("start", [0, 37, 6 * 16, 19 * 16])
+@pytest.mark.parametrize("bs", [16, 48])
+def test_bounds_of_a_chunk_end_with_its_table(dev, start, bs):
+    """With a table length, entries behind it are not read: their blocks keep what the buffer held."""
+    rng = np.random.default_rng(start + bs)
+    NBL, stride = 20, 6
+    p = R.Pool(rng, 1, 2, 4, 128, bs, NBL, cabi.BF16)
+    table = U.shuffled_table(rng, NBL, NBL)
+    db, dp, dt = G.bounds_dev(p), U.dev_bytes(p.raw), U.dev_i32(table)
+    db.fill_(0x55)
+    cabi.call("drk_kv_bounds_update", p.g, U.p(dp), U.p(dt), stride, None, start, 20 * bs - start - 3, 0, 1, U.p(db), U.stream_ptr())
+    U.sync()
+    codes, exps = G.bounds_host(p, db)
+    for lb in range(NBL):
+        if start // bs <= lb < stride:
+            G.check_block(p, codes, exps, 0, table[lb], bs)
+        else:
+            assert (codes[0, table[lb]] == 0x55).all() and (exps[0, table[lb]] == 0x55).all()
+
+
 # ---- attention --------------------------------------------------------------------------------
 class SinkPages:
     """Pages of one kv head in which the first token's key leads every other score by about `lead`, with a value of the

@@ -225,9 +225,13 @@ int drk_rope_apply(const drk_rope *r, const double *d_freqs, const drk_rope_rows
         if (x.heads > 0 && T > 1 && x.out_token_stride < (size_t)(x.heads - 1) * x.out_head_stride + head_dim &&
             (x.out_token_stride < (size_t)head_dim || x.heads == 1 || x.out_head_stride < (size_t)(T - 1) * x.out_token_stride + head_dim))
             return fail(DRK_ERR_INVALID, "rope_apply: tensor %d: rows of out overlap", i);
-        for (int j = 0; j < i; j++)
-            if (x.heads > 0 && tensors[j].heads > 0 && x.out == tensors[j].out)
-                return fail(DRK_ERR_INVALID, "rope_apply: tensors %d and %d have one output", j, i);
+        for (int j = 0; j < i; j++) {
+            if (x.heads <= 0 || tensors[j].heads <= 0) continue;
+            if (x.out == tensors[j].out) return fail(DRK_ERR_INVALID, "rope_apply: tensors %d and %d have one output", j, i);
+            // the tensors are rotated side by side: what one writes another must not read
+            if (x.out == tensors[j].x || x.x == tensors[j].out)
+                return fail(DRK_ERR_INVALID, "rope_apply: of tensors %d and %d one reads what the other writes", j, i);
+        }
         if (x.x == x.out && (x.x_token_stride != x.out_token_stride || x.x_head_stride != x.out_head_stride))
             return fail(DRK_ERR_INVALID, "rope_apply: tensor %d: in place needs equal strides", i);
         if (x.heads > (1 << 20)) return fail(DRK_ERR_INVALID, "rope_apply: tensor %d: %d heads", i, x.heads);

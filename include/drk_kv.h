@@ -492,8 +492,8 @@ int drk_rope_freqs_fill(const drk_rope *r, double *d_freqs, void *stream);
 int drk_rope_table_fill_scaled(const drk_rope *r, float *d_table, int n_pos, void *stream);
 /* One tensor of head rows: element (t, head, d) at t * token_stride + head * head_stride + d; strides in elements,
  * multiples of 8, pointers 16-byte aligned.  out may equal x with the same strides (in place); otherwise the two must
- * not overlap.  Rows of out must not overlap either, nor the out of two tensors of a call: tokens lie behind one
- * another's heads or heads behind one another's tokens. */
+ * not overlap.  Rows of out must not overlap either (tokens lie behind one another's heads or heads behind one another's
+ * tokens), nor the out of one tensor of a call with the x or the out of another: they are rotated side by side. */
 typedef struct drk_rope_rows {
     const void *x;
     void *out;

@@ -5,7 +5,7 @@ import ctypes as C
 import pytest
 
 from deusridet_amd import cabi, host
-from tests.test_longctx_refusals import code, lay
+from tests.test_longctx_refusals import P, code, lay, rope_code
 
 
 # ---- what the attention takes ------------------------------------------------------------------
@@ -43,3 +43,15 @@ def test_16_bit_pages_of_another_type_than_the_queries_are_not_supported():
         assert host.set_attention_geometry(2, 32, 8, 128, kv, io)
         assert host.lib().drkh_paged_sparse_attention_supported(16) and host_bytes(1, 4096, 64, 512, 16) > 0
         assert not any(host.lib().drkh_paged_sparse_attention_supported(b) for b in (0, 8, 24, -16))
+
+
+# ---- rotary positions ----------------------------------------------------------------------------
+def test_rope_refuses_tensors_of_which_one_reads_what_another_writes():
+    row = lambda x, out: (x * P, out * P, 8, 1024, 128, 1024, 128)
+    for rows in ([row(1, 2), row(2, 3)], [row(2, 3), row(1, 2)], [row(1, 2), row(2, 1)], [row(1, 1), row(1, 2)], [row(1, 2), row(1, 1)],
+                 [row(1, 2), row(3, 4), row(5, 1)]):
+        assert rope_code(rows=rows) == cabi.ERR_INVALID, rows
+        assert b"reads what" in cabi.lib().drk_last_error()
+    none = (P, 2 * P, 0, 1024, 128, 1024, 128)                              # without heads nothing is read or written
+    assert rope_code(rows=[none, (2 * P, 2 * P, 0, 0, 0, 0, 0)]) == cabi.OK
+    assert rope_code(rows=[row(1, 2), row(1, 3)], T=0) == cabi.OK           # two readers of one tensor

@@ -81,6 +81,32 @@ bool KvStream::init(CacheManager& cm, int max_context_len, ImportanceScorer* sco
     return true;
 }
 
+bool KvStream::set_scaled_rope(const drk_rope& rope, hipStream_t stream)
+{
+    if (!cm_) return false;
+    void* p = nullptr;
+    const size_t row = (size_t)ModelConfig::ROTARY_DIM * sizeof(float);
+    if (rope.rotary_dim != ModelConfig::ROTARY_DIM) {
+        LOG_ERROR("Conscientia", "KvStream: a rotary embedding of %d dims for a model of %d", rope.rotary_dim, ModelConfig::ROTARY_DIM);
+        return false;
+    }
+    if (drk_dev_malloc(&p, row * (size_t)max_context_len_) != DRK_OK ||
+        drk_rope_table_fill_scaled(&rope, static_cast<float*>(p), max_context_len_, stream) != DRK_OK ||
+        drk_stream_synchronize(stream) != DRK_OK) {           // the streams of the next calls find it there
+        LOG_ERROR("Conscientia", "KvStream: table of the stretched rotary positions: %s", drk_last_error());
+        if (p) drk_dev_free(p);
+        return false;
+    }
+    drop_graph();                                             // it reads the table it was recorded with
+    if (d_scaled_table_) {
+        drk_device_synchronize();                             // a launch may still be reading it
+        drk_dev_free(d_scaled_table_);
+    }
+    d_rope_table_ = d_scaled_table_ = static_cast<float*>(p);
+    table_positions_ = max_context_len_;
+    return true;
+}
+
 void KvStream::destroy()
 {
     drop_graph();
@@ -94,6 +120,11 @@ void KvStream::destroy()
         d_plan_ = nullptr;
     }
     plan_bytes_ = 0;
+    if (d_scaled_table_) {
+        drk_device_synchronize();                 // a launch may still be reading it
+        drk_dev_free(d_scaled_table_);
+        d_scaled_table_ = nullptr;
+    }
     if (d_row_lse_ || ev_attn_ || ev_mass_) {
         drk_device_synchronize();                 // a mass pass may still be reading
         if (d_row_lse_) drk_dev_free(d_row_lse_);

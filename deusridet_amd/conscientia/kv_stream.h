@@ -47,7 +47,9 @@ public:
     // cm must be initialised with max_branches >= 1 + the decode branches ever open at once.
     // scorer (optional): decode attention reports the attention mass per block into it; it must
     // cover cm.max_branches() * cm.table_stride() cells (init fails otherwise).
-    // d_rope_table (optional): see drk_rope_table_fill.
+    // d_rope_table (optional): see drk_rope_table_fill.  Positions beyond table_positions are rotated by the plain angles:
+    // a table of stretched ones that ends before max_context_len would turn the keys behind its end differently,
+    // unseen -- set_scaled_rope() brings one that does not.
     // max_prefill_rows: the longest chunk begin_prefill will be given.
     // Two workspaces for split-K partials are reserved here, one for perception and one for
     // decode, sized for max_context_len, every branch and max_prefill_rows: perception and decode
@@ -56,6 +58,11 @@ public:
     bool init(CacheManager& cm, int max_context_len, ImportanceScorer* scorer = nullptr,
               const float* d_rope_table = nullptr, int table_positions = 0, int max_prefill_rows = 2048);
     void destroy();
+    // Stretched rotary positions (drk_rope) in perception and decode, in place of init's table: the stream fills and keeps a
+    // table of its own for all max_context_len positions.  Half-half pairs, rotary_dim = ModelConfig::ROTARY_DIM.
+    // Call it before the first token (what is in the pages keeps its rotation); a captured step is dropped.  False, and
+    // nothing changes, where the description is refused or the table cannot be had.
+    bool set_scaled_rope(const drk_rope& rope, hipStream_t stream = nullptr);
 
     // ---- perception: the persistent stream, branch 0 -------------------------------------
     // May run between the decode steps of open branches (time division): the branches keep the
@@ -125,6 +132,7 @@ private:
     ImportanceScorer* scorer_ = nullptr;
     const float* d_rope_table_ = nullptr;
     int table_positions_ = 0;
+    float* d_scaled_table_ = nullptr;   // set_scaled_rope's, [max_context_len][ROTARY_DIM / 2][2]
     int max_context_len_ = 0;
     int current_pos_ = 0;
     std::vector<int> branches_;      // CacheManager branch ids of the open decode branches

@@ -104,6 +104,7 @@ SIGNATURES = {
     "drkh_kvs_branch_pos": (_i32, [_vp, _i32]),
     "drkh_kvs_shared_tokens": (_i32, [_vp]),
     "drkh_kvs_set_shared_prefix_policy": (None, [_vp, _i32, _i32]),
+    "drkh_kvs_set_scaled_rope": (_i32, [_vp, C.POINTER(cabi.Rope), _vp]),
     "drkh_kvs_set_sparse_decode": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp]),
     "drkh_kvs_begin_decode_step": (_i32, [_vp, _vp]),
     "drkh_kvs_decode_layer": (None, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
@@ -213,6 +214,7 @@ class KvStream:
     def set_branch_count(self, n): return lib().drkh_kvs_set_branch_count(self._h, n)
     def shared_tokens(self): return lib().drkh_kvs_shared_tokens(self._h)
     def set_shared_prefix_policy(self, min_branches, min_tokens): lib().drkh_kvs_set_shared_prefix_policy(self._h, min_branches, min_tokens)
+    def set_scaled_rope(self, rope, stream=None): return bool(lib().drkh_kvs_set_scaled_rope(self._h, rope, stream))
     def set_sparse_decode(self, min_tokens, n_keep, n_sink, n_recent, stream=None):
         return bool(lib().drkh_kvs_set_sparse_decode(self._h, min_tokens, n_keep, n_sink, n_recent, stream))
     def close_branches(self): lib().drkh_kvs_close_branches(self._h)

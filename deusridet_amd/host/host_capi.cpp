@@ -319,6 +319,7 @@ int drkh_kvs_init(void *ks, void *cm, int max_context_len, void *scorer, const f
 {
     return KS(ks)->init(*CM(cm), max_context_len, SC(scorer), d_rope_table, table_positions, max_prefill_rows) ? 1 : 0;
 }
+int drkh_kvs_set_scaled_rope(void *ks, const drk_rope *rope, void *stream) { return KS(ks)->set_scaled_rope(*rope, ST(stream)) ? 1 : 0; }
 int drkh_kvs_begin_prefill(void *ks, int M, void *stream) { return KS(ks)->begin_prefill(M, (hipStream_t)stream) ? 1 : 0; }
 void drkh_kvs_prefill_layer(void *ks, int fa_layer_idx, const void *qg, const void *k, const void *v, const void *q_norm,
                             const void *k_norm, void *q_scratch, void *attn_out, int M, void *stream)

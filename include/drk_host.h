@@ -185,6 +185,7 @@ int   drkh_kvs_branch_id(void *ks, int i);
 int   drkh_kvs_branch_pos(void *ks, int i);
 int   drkh_kvs_shared_tokens(void *ks);
 void  drkh_kvs_set_shared_prefix_policy(void *ks, int min_branches, int min_tokens);
+int   drkh_kvs_set_scaled_rope(void *ks, const struct drk_rope *rope, void *stream);
 int   drkh_kvs_set_sparse_decode(void *ks, int min_tokens, int n_keep, int n_sink, int n_recent, void *stream);
 int   drkh_kvs_begin_decode_step(void *ks, void *stream);
 void  drkh_kvs_decode_layer(void *ks, int fa_layer_idx, const void *qg, const void *k, const void *v, const void *q_norm,

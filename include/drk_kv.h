@@ -488,7 +488,8 @@ int drk_rope_freqs_fill(const drk_rope *r, double *d_freqs, void *stream);
 /* A cos/sin table for the entry points that take one (drk_apply_rope, drk_qk_norm_rope_append: half-half pairs,
  * rotary_dim = 16 * 2^k there): float [n_pos][rotary_dim/2][2] of magnitude * (cos, sin)(2 pi pos f'_i), the angle in
  * 64 bits and reduced before it is rounded.  Those entry points evaluate unstretched angles beyond the table: cover
- * every position. */
+ * every position (KvStream::set_scaled_rope does).  The table is formed from the description alone: frequencies of another
+ * kind -- a ramp over the pairs' indices, say -- are for drk_rope_apply, which takes any d_freqs. */
 int drk_rope_table_fill_scaled(const drk_rope *r, float *d_table, int n_pos, void *stream);
 /* One tensor of head rows: element (t, head, d) at t * token_stride + head * head_stride + d; strides in elements,
  * multiples of 8, pointers 16-byte aligned.  out may equal x with the same strides (in place); otherwise the two must

@@ -229,3 +229,41 @@ def test_select_from_more_than_a_million_blocks(dev, T, mode):
         s[:sink], s[lens[t] - recent:] = np.inf, np.inf
         want = np.sort(np.lexsort((np.arange(len(s)), -s))[:keep])
         assert np.array_equal(got[t, 0], want), t
+
+
+def test_the_driver_stretches_every_position_of_its_context(dev):
+    """set_scaled_rope: keys, queries and outputs are those of a table that covers the whole context, bit for bit, on both
+    sides of where init's own table ends; a refused description changes nothing."""
+    import torch
+    r = cabi.rope(S.RD, False, S.THETA, 8.0, 128.0, 1.0, 32.0, 1.2)
+
+    def session(own):
+        s = S.Session(2)
+        st = U.stream_ptr()
+        full = torch.zeros(S.NPOS * S.RD, dtype=torch.float32, device="cuda")
+        cabi.call("drk_rope_table_fill_scaled", r, U.p(full), S.NPOS, st)
+        assert s.ks.init(s.cm, S.NPOS, None, U.p(full), 48 if own else S.NPOS)
+        if own:
+            assert s.ks.set_scaled_rope(r, st)
+            for bad in (cabi.rope(2 * S.RD), cabi.rope(S.RD, True), cabi.rope(S.RD, factor=-1.0)):
+                assert not s.ks.set_scaled_rope(bad, st)
+        rng = np.random.default_rng(4)
+        s.set_weights(U.normal_bits(rng, (S.D,), S.DT), U.normal_bits(rng, (S.D,), S.DT))
+        SP.prefill(s, rng, (40, 20))
+        assert s.ks.open_branches(2) == 2
+        outs = []
+        for step in range(2):
+            assert s.ks.begin_decode_step(st)
+            for layer, x in enumerate(SP.step_inputs(rng, 2)):
+                s.load(*x)
+                s.ks.decode_layer(layer, s.io(), st)
+                outs.append(s.out(2))
+            s.ks.end_decode_step(st)
+        s.full = full
+        return s, outs
+
+    a, want = session(False)
+    b, got = session(True)
+    assert np.array_equal(a.pool(), b.pool())
+    assert all(np.array_equal(x, y) for x, y in zip(want, got))
+    assert not host.KvStream().set_scaled_rope(r)                        # not initialised

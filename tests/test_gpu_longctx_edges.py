@@ -11,6 +11,7 @@ from tests import test_gpu_longctx as G
 from tests import test_gpu_stream as S
 from tests import test_gpu_stream_sparse as SP
 from tests import util as U
+from tests.test_gpu_stream import eight_bit_pages  # noqa: F401 (a fixture: it changes the pages' type of S)
 
 pytestmark = pytest.mark.gpu
 
@@ -267,3 +268,41 @@ def test_the_driver_stretches_every_position_of_its_context(dev):
     assert np.array_equal(a.pool(), b.pool())
     assert all(np.array_equal(x, y) for x, y in zip(want, got))
     assert not host.KvStream().set_scaled_rope(r)                        # not initialised
+
+
+class View8:
+    """A session's pool bytes as float64 keys and values (8-bit pages), as longctx_ref's attention reads them."""
+
+    def __init__(self, s):
+        import torch
+        self.L, self.KVH, self.QH, self.D, self.bs, self.NB, self.dtype = S.L, S.KVH, S.QH, S.D, S.BS, s.NB, S.KVDT
+        raw = s.pool().reshape(S.L, s.NB, -1)
+        n = S.KVH * S.BS * S.D
+        codes = np.ascontiguousarray(raw[:, :, :2 * n])
+        if S.KVDT == cabi.INT8:
+            sc = np.ascontiguousarray(raw[:, :, 2 * n:2 * n + 4 * S.KVH * S.BS]).view(np.float16).astype(np.float64)
+            v = codes.view(np.int8).astype(np.float64).reshape(S.L, s.NB, 2, S.KVH, S.BS, S.D) * sc.reshape(S.L, s.NB, 2, S.KVH, S.BS, 1)
+        else:
+            v = torch.from_numpy(codes).view(torch.float8_e4m3fn).double().numpy().reshape(S.L, s.NB, 2, S.KVH, S.BS, S.D)
+        self.k, self.v = v[:, :, 0], v[:, :, 1]
+
+
+def test_the_driver_chooses_among_8_bit_pages(dev, eight_bit_pages, monkeypatch):
+    """Four of twelve blocks over int8 and fp8 pages: bounds, choice and attention of every step against the definitions."""
+    monkeypatch.setattr(SP, "View", View8)
+    s = S.Session(2)
+    st = U.stream_ptr()
+    rng = np.random.default_rng(14)
+    s.set_weights(U.normal_bits(rng, (S.D,), S.DT), U.normal_bits(rng, (S.D,), S.DT))
+    assert s.ks.set_sparse_decode(0, 4, 1, 1, st)
+    SP.prefill(s, rng, (64, 64, 50))
+    assert s.ks.open_branches(2) == 2
+    ids = [s.ks.branch_id(i) for i in range(2)]
+    for step in range(3):
+        assert s.ks.begin_decode_step(st)
+        pos = [s.ks.branch_pos(i) for i in range(2)]
+        for layer, x in enumerate(SP.step_inputs(rng, 2)):
+            s.load(*x)
+            s.ks.decode_layer(layer, s.io(), st)
+            SP.check_step(s, layer, ids, pos, x[0], s.out(2), 4, 1, 1)
+        s.ks.end_decode_step(st)

@@ -15,9 +15,15 @@
 namespace drk {
 
 constexpr int kBThreads = 256;
-// Tokens per block up to which a thread takes 16 bytes of every row of its unit; above, a workgroup takes a unit and folds
-// in LDS: blocks of 256 19 us instead of 36, blocks of 16 591 us instead of 43.
+// Which kernel: a thread takes 16 bytes of every row of its (layer, block, kv head), one row after the other (short), or a
+// workgroup takes the rows 16 per thread at once and folds in LDS (long).  The first takes as long as a block has rows, the
+// second as long as there are units, for 64 KiB of loads each, those beyond the unit's last row repeated.  Us, short / long:
+//   few units, 8 branches x 8 heads:  bf16 x 128, blocks of 32 4.3 / 4.3, 64 6.0 / 4.2, 256 16.7 / 4.2; int8 32 7.4 / 7.1, 64 11.9 / 7.1
+//   131 072 tokens x 8 heads, int8 x 128:  blocks of 32 26 / 398, 64 24 / 205, 128 30 / 105, 256 52 / 61
+//   65 536 tokens x 8 heads, bf16 x 128:   blocks of 32 22 / 64, 64 21 / 32, 128 22 / 22, 256 31 / 21
+// So: the long one for blocks above 32 tokens where the units are fewer than a unit's 16-byte chunks, or a unit fills the loads.
 constexpr int kBLongBlock = 32;
+constexpr size_t kBLongBytes = 64 << 10;
 
 struct BoundsArgs {
     const uint8_t *pool;
@@ -133,7 +139,7 @@ __device__ __forceinline__ uint32_t bounds_code(float x, int e, bool high)
     return (uint32_t)(int)(high ? ceilf(y) : floorf(y)) & 0xffu;
 }
 
-// Short blocks: a thread owns 16 bytes of every row of its unit, so nothing is exchanged but the largest magnitude;
+// Many or short units: a thread owns 16 bytes of every row of its unit, so nothing is exchanged but the largest magnitude;
 // row_bytes / 16 neighbouring lanes hold a unit.
 template <int DT>
 __global__ __launch_bounds__(kBThreads) void bounds_update_kernel(Lay a, BoundsArgs A, unsigned lpr, int lpr_shift)
@@ -177,7 +183,7 @@ __global__ __launch_bounds__(kBThreads) void bounds_update_kernel(Lay a, BoundsA
     if (sub == 0) A.bounds[A.exps + entry] = (uint8_t)(int8_t)e;
 }
 
-// Long blocks: a workgroup per unit, its rows dealt out to 256 / lpr threads per 16-byte column; the partial bounds meet
+// Few or long units: a workgroup per unit, its rows dealt out to 256 / lpr threads per 16-byte column; the partial bounds meet
 // in LDS, where thread d then owns dimension d.
 template <int DT>
 __global__ __launch_bounds__(kBThreads) void bounds_update_long_kernel(Lay a, BoundsArgs A, unsigned lpr, int lpr_shift)
@@ -305,7 +311,8 @@ int drk_kv_bounds_update(const drk_kv_layout *g, const void *pool, const int32_t
     A.units = (unsigned)units;
     const unsigned lpr = a.row_bytes / 16;
     const int lpr_shift = ilog2_exact(lpr);
-    const bool wide = a.bs > kBLongBlock;
+    const size_t unit_bytes = (size_t)a.bs * a.row_bytes;
+    const bool wide = a.bs > kBLongBlock && (units <= unit_bytes / 16 || unit_bytes >= kBLongBytes);
     const dim3 grid(wide ? (unsigned)units : (unsigned)((units * lpr + kBThreads - 1) / kBThreads));
     hipStream_t st = (hipStream_t)stream;
 #define DRK_BOUNDS_LAUNCH(DT)                                                                                             \

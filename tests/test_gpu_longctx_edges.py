@@ -62,6 +62,26 @@ def test_bounds_of_a_chunk_end_with_its_table(dev, start, bs):
             assert (codes[0, table[lb]] == 0x55).all() and (exps[0, table[lb]] == 0x55).all()
 
 
+@pytest.mark.parametrize("dtype", G.DTYPES)
+@pytest.mark.parametrize("D,bs,NBL", [(64, 48, 150), (128, 64, 180), (64, 256, 280), (256, 40, 240)])
+def test_bounds_of_many_long_blocks(dev, dtype, D, bs, NBL):
+    """Blocks above 32 tokens in such numbers that a thread walks every row of its columns; the last one is cut."""
+    rng = np.random.default_rng(D + bs)
+    p = R.Pool(rng, 2, 4, 4, D, bs, NBL, dtype)
+    assert 2 * 4 * NBL * 16 > bs * D * (1 if dtype in (cabi.INT8, cabi.FP8_E4M3) else 2)
+    table = U.shuffled_table(rng, NBL, NBL)
+    last = bs - 5
+    for layer in range(2):
+        p.poison(layer, table[-1], last)
+    db, dp, dt = G.bounds_dev(p), U.dev_bytes(p.raw), U.dev_i32(table)
+    cabi.call("drk_kv_bounds_update", p.g, U.p(dp), U.p(dt), NBL, None, 0, NBL * bs - 5, 0, 2, U.p(db), U.stream_ptr())
+    U.sync()
+    codes, exps = G.bounds_host(p, db)
+    for lb in (0, 1, 2, 37, NBL // 2, NBL - 2, NBL - 1):
+        for layer in range(2):
+            G.check_block(p, codes, exps, layer, table[lb], bs if lb < NBL - 1 else last)
+
+
 # ---- attention --------------------------------------------------------------------------------
 class SinkPages:
     """Pages of one kv head in which the first token's key leads every other score by about `lead`, with a value of the

@@ -4,6 +4,7 @@
 #include "drk_host.h"
 
 #include "../machina/paged_attention.h"
+#include "../communis/log.h"
 #include "../machina/layer.h"
 #include "../memoria/kv_swapper.h"
 #include "../conscientia/kv_stream.h"
@@ -243,6 +244,10 @@ void drkh_apply_rope(void *q, void *k, int num_heads, int num_kv_heads, int head
 void drkh_apply_rope_scaled(const drk_rope *rope, const double *d_freqs, void *q, void *k, int T, int num_heads, int num_kv_heads,
                             int head_dim, const int32_t *d_pos, int pos_start, int inverse, void *stream)
 {
+    if (!rope) {
+        LOG_ERROR("Machina", "apply_rope_scaled: no description");
+        return;
+    }
     apply_rope_scaled(*rope, d_freqs, H(q), H(k), T, num_heads, num_kv_heads, head_dim, d_pos, pos_start, inverse != 0, ST(stream));
 }
 int drkh_paged_sparse_attention_supported(int block_size) { return paged_sparse_attention_supported(block_size) ? 1 : 0; }
@@ -319,7 +324,7 @@ int drkh_kvs_init(void *ks, void *cm, int max_context_len, void *scorer, const f
 {
     return KS(ks)->init(*CM(cm), max_context_len, SC(scorer), d_rope_table, table_positions, max_prefill_rows) ? 1 : 0;
 }
-int drkh_kvs_set_scaled_rope(void *ks, const drk_rope *rope, void *stream) { return KS(ks)->set_scaled_rope(*rope, ST(stream)) ? 1 : 0; }
+int drkh_kvs_set_scaled_rope(void *ks, const drk_rope *rope, void *stream) { return rope && KS(ks)->set_scaled_rope(*rope, ST(stream)) ? 1 : 0; }
 int drkh_kvs_begin_prefill(void *ks, int M, void *stream) { return KS(ks)->begin_prefill(M, (hipStream_t)stream) ? 1 : 0; }
 void drkh_kvs_prefill_layer(void *ks, int fa_layer_idx, const void *qg, const void *k, const void *v, const void *q_norm,
                             const void *k_norm, void *q_scratch, void *attn_out, int M, void *stream)

@@ -55,3 +55,10 @@ def test_rope_refuses_tensors_of_which_one_reads_what_another_writes():
     none = (P, 2 * P, 0, 1024, 128, 1024, 128)                              # without heads nothing is read or written
     assert rope_code(rows=[none, (2 * P, 2 * P, 0, 0, 0, 0, 0)]) == cabi.OK
     assert rope_code(rows=[row(1, 2), row(1, 3)], T=0) == cabi.OK           # two readers of one tensor
+
+
+def test_the_host_functions_take_no_missing_description():
+    """NULL for a description: refused (an uninitialised driver and no tensors: nothing is launched either way)."""
+    h = host.lib()
+    h.drkh_apply_rope_scaled(None, P, P, P, 1, 8, 2, 128, None, 0, 0, None)
+    assert host.KvStream().set_scaled_rope(None) is False
